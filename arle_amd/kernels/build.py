@@ -54,10 +54,14 @@ SOURCES = {
     "decay_scan": "decay_scan.hip",
     "gated_linear": "gated_linear.hip",
     "state_space": "state_space.hip",
+    "mx_rows": "mx_rows.hip",
+    "mx_gemm": "mx_gemm.hip",
     "host": "host/runtime.cpp",
 }
 HEADERS = ("common.h", "once_a_device.h", "attention_static.h", "attention_args.h", "attention_stream.h", "attention_portions.h",
            "attention_portions_dma.h", "lds_loads.h", "attention_softcap_portions.h", "addend.h", "chunks.h", "lane_sums.h", "scaled_rows.h")
+# headers that only some sources include: they count for those alone, so that a change compiles no other library again
+OWN_HEADERS = {"mx_rows": ("mx.h",), "mx_gemm": ("mx.h",)}
 HOST_LIBS = ("host",)   # plain C++: page pool, block tables, step packing
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared"]
 
@@ -141,7 +145,7 @@ def find_host_compiler() -> str:
 def source_hash(name: str) -> str:
     h = hashlib.sha256()
     host = name in HOST_LIBS
-    for fname in ((SOURCES[name],) if host else (SOURCES[name], *HEADERS)):
+    for fname in ((SOURCES[name],) if host else (SOURCES[name], *HEADERS, *OWN_HEADERS.get(name, ()))):
         with open(os.path.join(CSRC_DIR, fname), "rb") as fh:
             h.update(fh.read())
     h.update(" ".join(HOST_FLAGS if host else HIPCC_FLAGS).encode())

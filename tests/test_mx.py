@@ -1,0 +1,156 @@
+"""Microscaled rows and weights on the host: layouts of weights, and the calls that the entry points refuse before anything is launched."""
+import pytest
+import torch
+
+import plain_mx as plain
+from arle_amd.kernels import lib, mx, ops
+
+
+@pytest.fixture
+def no_gpu(monkeypatch):
+    """CPU tensors pass, and no kernel may be asked for."""
+    monkeypatch.setattr(mx, "_here", lambda *t: None)
+
+    def call(name, *args):
+        raise AssertionError(f"{name} was launched")
+
+    monkeypatch.setattr(lib, "call", call)
+
+
+def _rows(T, width, form="mxfp8", seed=0):
+    g = torch.Generator().manual_seed(seed)
+    e = torch.randint(0, 16 if form == "mxfp4" else 120, (T, width), generator=g, dtype=torch.uint8)
+    s = torch.randint(100, 140, (T, -(-width // 32)), generator=g, dtype=torch.uint8)
+    return e, s, mx.rows_from_codes(e, s, width, form)
+
+
+@pytest.mark.parametrize("form", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("T,width", [(0, 32), (1, 1), (3, 255), (5, 256), (2, 257), (4, 700)])
+def test_rows_from_codes(no_gpu, form, T, width):
+    e, s, rows = _rows(T, width, form)
+    assert rows.rows == T and rows.padded % 256 == 0 and 0 <= rows.padded - width < 256
+    got_e, got_s = plain.unpack(rows)
+    assert torch.equal(got_e[:, :width], e) and not got_e[:, width:].any()
+    blocks = s.shape[1]
+    assert torch.equal(got_s[:, :blocks], s) and not got_s[:, blocks:].any()
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (17, 129), (40, 700), (33, 1100)])
+def test_weight_tiles(no_gpu, n, k):
+    """Lane 16 g + i of tile (t, s) holds row 16 t + i, k 128 s + 32 g ..; byte s % 4 of its scale word is that block's."""
+    e, s, rows = _rows(n, k, "mxfp4")
+    w = mx.lay_weight(rows)
+    assert (w.n, w.k, w.gated) == (n, k, False)
+    codes, scales = plain.unpack(rows)
+    for t in range(w.tiles.shape[0]):
+        for st in range(w.tiles.shape[1]):
+            for lane in range(64):
+                g, i = divmod(lane, 16)
+                row = 16 * t + i
+                piece = w.tiles[t, st, lane]
+                got = torch.stack([piece & 15, piece >> 4], dim=-1).flatten()
+                at = 128 * st + 32 * g
+                want = codes[row, at:at + 32] if row < n else torch.zeros(32, dtype=torch.uint8)
+                assert torch.equal(got, want)
+                assert w.scales[t, st // 4, lane, st % 4] == (scales[row, at // 32] if row < n else 0)
+
+
+@pytest.mark.parametrize("ff", [1, 16, 100, 256, 300])
+def test_gated_weight_is_turns_of_sixteen(no_gpu, ff):
+    e, s, rows = _rows(2 * ff, 64, "mxfp4")
+    w = mx.lay_weight(rows, gated=True)
+    padded = -(-ff // 256) * 256
+    assert w.n == 2 * ff and w.tiles.shape[0] == 2 * padded // 16
+    codes, _ = plain.unpack(rows)
+    for c in range(0, padded, 7):
+        for which in (0, 1):
+            piece = w.tiles[2 * (c // 16) + which, 0, c % 16]
+            got = torch.stack([piece & 15, piece >> 4], dim=-1).flatten()
+            assert torch.equal(got, codes[which * ff + c, :32] if c < ff else torch.zeros(32, dtype=torch.uint8))
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 64)
+    for call in (lambda: mx.quantize(x), lambda: mx.add_rmsnorm(x, None, torch.ones(64), 1e-6),
+                 lambda: mx.rows_from_codes(torch.zeros(2, 64, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8), 64, "mxfp8")):
+        with pytest.raises(ops.ShapeError, match="GPU only"):
+            call()
+
+
+def test_refused_rows(no_gpu):
+    bad = [
+        lambda: mx.quantize(torch.zeros(2, 64), "mxfp6"),
+        lambda: mx.quantize(torch.zeros(2, 64, dtype=torch.float16)),
+        lambda: mx.quantize(torch.zeros(64)),
+        lambda: mx.quantize(torch.zeros(2, 0)),
+        lambda: mx.quantize(torch.zeros(64, 4).T),                                      # columns apart
+        lambda: mx.rows_from_codes(torch.zeros(2, 64, dtype=torch.uint8), torch.zeros(2, 3, dtype=torch.uint8), 64, "mxfp8"),
+        lambda: mx.rows_from_codes(torch.zeros(2, 63, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8), 64, "mxfp8"),
+        lambda: mx.rows_from_codes(torch.full((2, 64), 16, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8), 64, "mxfp4"),
+        lambda: mx.rows_from_codes(torch.zeros(2, 64), torch.zeros(2, 2, dtype=torch.uint8), 64, "mxfp8"),
+        lambda: _rows(2, 64, "mxfp4")[2].elements_e4m3(),
+        lambda: mx.values(torch.zeros(2, 64)),
+        lambda: mx.values(_rows(2, 64)[2], torch.float16),
+        lambda: mx.values(mx.MXRows(torch.zeros(2, 300, dtype=torch.uint8)[:, 1:257], torch.zeros(2, 8, dtype=torch.uint8), 256, "mxfp8")),
+        lambda: mx.values(mx.MXRows(torch.zeros(2, 256, dtype=torch.uint8), torch.zeros(2, 8, dtype=torch.uint8), 300, "mxfp8")),
+        lambda: mx.values(mx.MXRows(torch.zeros(2, 256, dtype=torch.uint8), torch.zeros(1, 8, dtype=torch.uint8), 256, "mxfp8")),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ops.ShapeError):
+            call()
+            pytest.fail(f"call {i} passed")
+
+
+def test_refused_norms(no_gpu):
+    res, w = torch.zeros(3, 64), torch.ones(64)
+    bad = [
+        lambda: mx.add_rmsnorm(res.bfloat16(), None, w, 1e-6),
+        lambda: mx.add_rmsnorm(res[:, :32], None, w[:32], 1e-6),
+        lambda: mx.add_rmsnorm(res, res[:2], w, 1e-6),
+        lambda: mx.add_rmsnorm(res, torch.zeros(0, 3, 64), w, 1e-6),
+        lambda: mx.add_rmsnorm(res, res.half(), w, 1e-6),
+        lambda: mx.add_rmsnorm(res, None, w[:63], 1e-6),
+        lambda: mx.add_rmsnorm(res, None, w.half(), 1e-6),
+        lambda: mx.add_rmsnorm(res, None, w, 1e-6, "fp8"),
+        lambda: mx.add_rmsnorm(res, None, w, 1e-6, rows=torch.zeros(2, dtype=torch.int64)),
+        lambda: mx.add_rmsnorm(torch.zeros(1, mx.MAX_WIDTH + 1), None, torch.ones(mx.MAX_WIDTH + 1), 1e-6),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ops.ShapeError):
+            call()
+            pytest.fail(f"call {i} passed")
+
+
+def test_refused_products(no_gpu):
+    x = _rows(3, 300)[2]
+    w = mx.lay_weight(_rows(40, 300, "mxfp4")[2])
+    wg = mx.lay_weight(_rows(40, 300, "mxfp4")[2], gated=True)
+    bad = [
+        lambda: mx.lay_weight(_rows(40, 300)[2]),                        # weights are held in 4 bits
+        lambda: mx.lay_weight(_rows(0, 300, "mxfp4")[2]),
+        lambda: mx.lay_weight(_rows(41, 300, "mxfp4")[2], gated=True),
+        lambda: mx.gemm(torch.zeros(3, 300), w),
+        lambda: mx.gemm(x, torch.zeros(40, 300)),
+        lambda: mx.gemm(x, wg),
+        lambda: mx.gate_up_act(x, w),
+        lambda: mx.gate_up_act(x, wg, "fp4"),
+        lambda: mx.gemm(_rows(3, 299)[2], w),
+        lambda: mx.gemm(x, w, torch.float16),
+        lambda: mx.gemm(x, mx.MXWeight(w.tiles[:1], w.scales, 40, 300)),
+        lambda: mx.gemm(x, mx.MXWeight(w.tiles, w.scales, 60, 300)),
+        lambda: mx.gemm(_rows(17, 300)[2], w, variant=0),                # more rows than the kernel holds
+        lambda: mx.gemm(x, w, variant=0, splits=5),                      # four steps of 128
+        lambda: mx.gemm(_rows(3, 300, "mxfp4")[2], w, variant=3, splits=3),   # two steps of 256
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ops.ShapeError):
+            call()
+            pytest.fail(f"call {i} passed")
+
+
+def test_no_rows_launch_nothing(no_gpu):
+    w, wg = mx.lay_weight(_rows(40, 300, "mxfp4")[2]), mx.lay_weight(_rows(40, 300, "mxfp4")[2], gated=True)
+    none = _rows(0, 300)[2]
+    assert mx.gemm(none, w).shape == (0, 40) and mx.gate_up_act(none, wg).rows == 0
+    assert mx.quantize(torch.zeros(0, 64)).rows == 0 and mx.values(none).shape == (0, 300)
+    assert mx.add_rmsnorm(torch.zeros(0, 64), None, torch.ones(64), 1e-6).rows == 0
