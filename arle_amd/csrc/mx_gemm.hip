@@ -4,7 +4,7 @@
 //
 // W is laid out once as operand tiles of 16 columns x 128 k, [ceil(N/16)][K/128][64][16 bytes], lane 16 g + i: W[16 t + i][128 s + 32 g
 // .. + 31], one contiguous kilobyte a wave and load; its scales as [ceil(N/16)][ceil(K/512)][64] words, byte s % 4 of lane 16 g + i
-// for that lane's block of tile s.  K is padded with zeros to a multiple of 256 on both sides.
+// for that lane's block of tile s.  K is padded with zeros to a multiple of 512 on both sides.
 //
 // With W as the first operand (rows of the result are W's columns) a lane ends up with four neighbouring columns of one row.
 // Operand layouts of the second operand's lane (row i, group g): e2m1 32 neighbouring k from 32 g on, as the first; e4m3 16 neighbouring
@@ -12,6 +12,7 @@
 // lane group g's byte is the scale of block g.  With e4m3 the instruction aligns the products of 8 neighbouring k to the largest of
 // them and drops what is under 2^-13 of it (measured with pairs of products); everything behind that is 32 bits wide.  That is 2^-9
 // of what rounding to e4m3 has taken from a number before.
+#include "lds_loads.h"
 #include "mx.h"
 
 #include <type_traits>
@@ -46,7 +47,11 @@ __device__ __forceinline__ mx_i32x8 mx_operand8(u32x4 a, u32x4 b) {
   return mx_i32x8{static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]),
                   static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3])};
 }
-__device__ __forceinline__ float mx_silu_mul(float gate, float up) { return gate / (1.0f + expf(-gate)) * up; }
+// silu(gate) * up by the hardware's exponential and reciprocal, a step of 32 bits off each: a 2^-18th of what the rounding to an element of 8 bits
+// takes.  (With expf and the exact quotient the activations of a workgroup's 256 x 128 results were a tenth of its time at K = 4,096.)
+__device__ __forceinline__ float mx_silu_mul(float gate, float up) {
+  return gate * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(gate * -1.44269504088896340736f)) * up;
+}
 
 template <int EPI>
 __device__ __forceinline__ void mx_store_sums(const MxArgs& a, int split, int row, int n, mx_f32x4 v) {
@@ -72,20 +77,23 @@ __device__ __forceinline__ void mx_store_sums(const MxArgs& a, int split, int ro
   }
 }
 
-// ---- few rows: W is streamed once
+// ---- up to 16 rows: W is streamed once
 //
-// A workgroup owns CT column tiles and a part of K (blockIdx.y); its WAVES waves take the part's tiles in turn and add their sums
-// through LDS in the order of the waves.  X comes from the caches, straight into operands.
-template <int BITS, int RT, int CT, int WAVES, int U, int EPI>
+// A workgroup owns CT column tiles and a part of K (blockIdx.y); its WAVES waves take the part's tiles in turn, kMxAhead on their way, and add
+// their sums through LDS in the order of the waves.  X comes from the caches, straight into operands.  Every condition is the same
+// in a whole wave, and no tile is fetched twice: loads past the end, though they hit the caches, were 2 of 13 us.
+constexpr int kMxAhead = 5;
+
+template <int BITS, int CT, int WAVES, int EPI>
 __global__ __launch_bounds__(WAVES* kWave) void mx_gemm_rows_kernel(const MxArgs a) {
-  constexpr bool kGate = EPI == kMxGate8 || EPI == kMxGate4;
-  static_assert(!kGate || CT == 4, "a block of 32 results is two tiles of gate and two of up columns");
+  constexpr int PD = kMxAhead, kParts = BITS == kMx8 ? 2 : 1;
   constexpr int kSub = 17, kTile = 4 * kSub;      // places of a tile's four columns x 16 rows, padded against bank conflicts
-  __shared__ mx_f32x4 parts[WAVES][RT * CT][kTile];
+  __shared__ mx_f32x4 parts[WAVES][CT][kTile];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4;
-  const int ct0 = blockIdx.x * CT, k_tiles = a.k_tiles, k_groups = (k_tiles + 3) / 4;
+  const int ct0 = blockIdx.x * CT, k_tiles = a.k_tiles, k_groups = k_tiles / 4;
   const int begin = blockIdx.y * a.per_split, end = min(begin + a.per_split, k_tiles);
+  const int n = (end - begin - wave + WAVES - 1) / WAVES;      // this wave's tiles: begin + wave, + WAVES, ...; none or less: none
 
   const uint8_t* wp[CT];
   const uint32_t* wsp[CT];
@@ -95,124 +103,90 @@ __global__ __launch_bounds__(WAVES* kWave) void mx_gemm_rows_kernel(const MxArgs
     wp[c] = a.w + tile * k_tiles * 1024 + lane * 16;
     wsp[c] = a.ws + tile * k_groups * 64 + lane;
   }
-  const uint8_t* xp[RT];
-  const uint8_t* xsp[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int64_t row = min(16 * r + i, a.M - 1);
-    xp[r] = a.x + row * a.ldx + 16 * g;
-    xsp[r] = a.xs + row * a.ldxs;
-  }
+  const int64_t row = min(i, a.M - 1);                          // lanes past the rows: the last row again, their sums are dropped
+  const uint8_t* xp = a.x + row * a.ldx + 16 * g;
+  const uint8_t* xsp = a.xs + row * a.ldxs;
   struct Step {
-    u32x4 w[CT], x[RT][BITS == kMx8 ? 2 : 1];
-    uint32_t ws[CT], xs[RT];
+    u32x4 w[CT], x[kParts];
+    uint32_t ws[CT], xs;
   };
   auto load = [&](int t, Step& s) {
-    t = min(t, end - 1);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       s.w[c] = *reinterpret_cast<const u32x4*>(wp[c] + static_cast<int64_t>(t) * 1024);
       s.ws[c] = wsp[c][(t >> 2) * 64];
     }
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      if constexpr (BITS == kMx8) {
-        s.x[r][0] = *reinterpret_cast<const u32x4*>(xp[r] + static_cast<int64_t>(t) * 128);
-        s.x[r][1] = *reinterpret_cast<const u32x4*>(xp[r] + static_cast<int64_t>(t) * 128 + 64);
-      } else {
-        s.x[r][0] = *reinterpret_cast<const u32x4*>(xp[r] + static_cast<int64_t>(t) * 64);
-      }
-      s.xs[r] = *reinterpret_cast<const uint32_t*>(xsp[r] + 4 * t);
-    }
+    for (int half = 0; half < kParts; ++half) s.x[half] = *reinterpret_cast<const u32x4*>(xp + static_cast<int64_t>(t) * (16 * BITS) + 64 * half);
+    s.xs = *reinterpret_cast<const uint32_t*>(xsp + 4 * t);
   };
-  mx_f32x4 acc[RT][CT];
+  mx_f32x4 acc[CT];
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int c = 0; c < CT; ++c) acc[r][c] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < CT; ++c) acc[c] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](int t, const Step& s) {
-    if (t >= end) return;     // the same in all lanes
+    mx_i32x8 xo;
+    if constexpr (BITS == kMx8)
+      xo = mx_operand8(s.x[0], s.x[1]);
+    else
+      xo = mx_operand4(s.x[0]);
+    const int xscale = static_cast<int>(s.xs >> (8 * g));
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      mx_i32x8 xo;
-      if constexpr (BITS == kMx8)
-        xo = mx_operand8(s.x[r][0], s.x[r][1]);
-      else
-        xo = mx_operand4(s.x[r][0]);
-      const int xscale = static_cast<int>(s.xs[r] >> (8 * g));
-#pragma unroll
-      for (int c = 0; c < CT; ++c)
-        acc[r][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand4(s.w[c]), xo, acc[r][c], 4, BITS == kMx8 ? 0 : 4, 0,
-                                                                     static_cast<int>(s.ws[c] >> (8 * (t & 3))), 0, xscale);
-    }
+    for (int c = 0; c < CT; ++c)
+      acc[c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand4(s.w[c]), xo, acc[c], 4, BITS == kMx8 ? 0 : 4, 0,
+                                                                static_cast<int>(s.ws[c] >> (8 * (t & 3))), 0, xscale);
   };
-  Step now[U], next[U];
-  int t = begin + wave;
+  Step ring[PD];
 #pragma unroll
-  for (int u = 0; u < U; ++u) load(t + u * WAVES, now[u]);
-  while (t < end) {
+  for (int u = 0; u < PD; ++u)
+    if (u < n) load(begin + wave + u * WAVES, ring[u]);
+  for (int s0 = 0; s0 < n; s0 += PD) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) load(t + (U + u) * WAVES, next[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) multiply(t + u * WAVES, now[u]);
-    t += U * WAVES;
-    if (t >= end) break;
-#pragma unroll
-    for (int u = 0; u < U; ++u) load(t + (U + u) * WAVES, now[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) multiply(t + u * WAVES, next[u]);
-    t += U * WAVES;
+    for (int u = 0; u < PD; ++u) {
+      const int s = s0 + u, t = begin + wave + s * WAVES;
+      if (s < n) multiply(t, ring[u]);
+      if (s + PD < n) load(t + PD * WAVES, ring[u]);
+    }
   }
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int c = 0; c < CT; ++c) parts[wave][r * CT + c][g * kSub + i] = acc[r][c];
+  for (int c = 0; c < CT; ++c) parts[wave][c][g * kSub + i] = acc[c];
   __syncthreads();
-
-  auto sum = [&](int tile, int at) {
-    mx_f32x4 s = parts[0][tile][at];
+  for (int item = tid; item < 16 * CT * 4; item += WAVES * kWave) {      // (row, four columns)
+    const int r = item / (CT * 4), q = item % (CT * 4), at = (q & 3) * kSub + r;
+    mx_f32x4 sum = parts[0][q >> 2][at];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) s += parts[w][tile][at];
-    return s;
-  };
-  if constexpr (kGate) {
-    for (int item = tid; item < RT * 16 * 8; item += WAVES * kWave) {     // (row, four of 32 results): eight lanes a block
-      const int row = item >> 3, q = item & 7, tile = (row >> 4) * CT + 2 * (q >> 2), at = (q & 3) * kSub + (row & 15);
-      const mx_f32x4 gate = sum(tile, at), up = sum(tile + 1, at);
-      const float4 v = {mx_silu_mul(gate[0], up[0]), mx_silu_mul(gate[1], up[1]), mx_silu_mul(gate[2], up[2]), mx_silu_mul(gate[3], up[3])};
-      constexpr int kBits = EPI == kMxGate8 ? kMx8 : kMx4;
-      const uint32_t code = mx_code<kBits>(mx_lanes_max<8>(mx_max4(v)));
-      if (row < a.M) {
-        mx_store4<kBits>(static_cast<uint8_t*>(a.out) + row * a.ldo, 32 * blockIdx.x + 4 * q, mx_pack4<kBits>(v, code));
-        if (q == 0) a.out_scales[row * a.ldos + blockIdx.x] = static_cast<uint8_t>(code);
-      }
-    }
-  } else {
-    for (int item = tid; item < RT * 16 * CT * 4; item += WAVES * kWave) {
-      const int row = item / (CT * 4), q = item % (CT * 4);
-      mx_store_sums<EPI>(a, blockIdx.y, row, 16 * ct0 + 4 * q, sum((row >> 4) * CT + (q >> 2), (q & 3) * kSub + (row & 15)));
-    }
+    for (int w = 1; w < WAVES; ++w) sum += parts[w][q >> 2][at];
+    mx_store_sums<EPI>(a, blockIdx.y, r, 16 * ct0 + 4 * q, sum);
   }
 }
 
 // ---- many rows
 //
-// A workgroup of RW x CW waves owns 32 MT RW rows and 32 TN CW columns; a wave 32 MT rows and 32 TN columns.  A step is 128 bytes of
-// every row of X: 128 k of e4m3, 256 of e2m1.  X goes through registers into LDS, rows of 128 bytes whose 16-byte pieces are
-// exchanged by the row (piece c of row r at c ^ (r % 8)), so that neither the lanes that park a row nor the lanes that read a
-// column of pieces share banks; two stages.  W goes straight from its tiles into operands, PD steps ahead.
-template <int BITS, int MT, int TN, int RW, int CW, int PD, int EPI>
-__global__ __launch_bounds__(RW* CW* kWave) void mx_gemm_tiles_kernel(const MxArgs a) {
+// A workgroup of RW x CW waves owns 32 MT RW rows and 32 TN CW columns; a wave 32 MT rows and 32 TN columns.  A step is 128 k; a round is
+// 512 k, for which scales come as 16 bytes a row of X and a word a lane of W.
+//
+// Everything goes from memory straight into LDS (load_to_lds_16), STAGES steps in turn, and from there into operands: no load of the
+// loop passes through registers, so that the only waits for memory are the counted ones in front of a step's barrier.
+//   * X: rows of 128 or 64 bytes, 16-byte pieces exchanged by the row: piece c of row r at c ^ (r / 2 % 8), or c ^ (r / 4 % 4), so that neighbouring
+//     lanes fetch a row's contiguous bytes and sixteen lanes that read a column of pieces meet all 64 banks.
+//   * W: its tiles as they are, a kilobyte a load; a 32-column operand is two tiles' runs of 256 bytes.
+//   * A step is 2 MT groups of TN products.  In every group the operands of the next group are read and a few of the batch's loads are sent, in
+//     an order that is pinned (left to itself the compiler gathers two steps' reads in front of two steps' products).  The step's
+//     barrier stands before its last group, whose operands are in registers: behind it the next step's stage is there and this
+//     step's is free, and the next step's first operands are read while the last products run.
+template <int BITS, int MT, int TN, int RW, int CW, int STAGES, int WAVES_A_SIMD, int EPI>
+__global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_kernel(const MxArgs a) {
   constexpr bool kGate = EPI == kMxGate8 || EPI == kMxGate4;
-  static_assert(!kGate || TN == 2, "a block of 32 results is two tiles of 16 gate and 16 up columns");
-  static_assert(PD % 2 == 0, "the stage alternates inside a round");
-  constexpr int kThreads = RW * CW * kWave, kRows = 32 * MT * RW;
-  constexpr int KT = BITS == kMx8 ? 1 : 2, KK = 2 * KT;      // tiles of 128 k and halves of 64 k in a step
-  constexpr int kStage = kRows * (128 + 4 * KT);
-  constexpr int XH = kRows * 8 / kThreads;
-  static_assert(XH * kThreads == kRows * 8 && kRows <= kThreads * 2, "whole pieces a thread");
-  constexpr int XS = (kRows + kThreads - 1) / kThreads;      // rows whose scales a thread parks
+  static_assert(!kGate || TN % 2 == 0, "a block of 32 results is two tiles of 16 gate and 16 up columns");
+  constexpr int kWaves = RW * CW, kRows = 32 * MT * RW, kTiles = 2 * TN * CW;
+  constexpr int kRowBytes = 16 * BITS, kPieces = kRowBytes / 16, kRowsALoad = 64 / kPieces;
+  constexpr int kXBytes = kRows * kRowBytes, kStage = kXBytes + kTiles * 1024;
+  constexpr int kXScales = (kRows < 64 ? 64 : kRows) * 16, kScales = kXScales + kTiles * 256;   // of a round
+  constexpr int XD = kXBytes / 1024 / kWaves, WD = kTiles / kWaves, kBatch = XD + WD;   // loads of a wave and step
+  constexpr int kGroups = 2 * MT;
+  static_assert(XD * kWaves * 1024 == kXBytes && WD * kWaves == kTiles && kTiles % 4 == 0, "whole loads a wave");
+  static_assert(STAGES >= 2 && STAGES <= 8, "a step's batch is sent STAGES - 1 steps ahead; a ninth would overtake a round's scales");
   extern __shared__ __align__(16) unsigned char lds[];
+  unsigned char* const lds_scales = lds + STAGES * kStage;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane & 31, h = lane >> 5;
   const int wr = wave / CW, wc = wave % CW;
@@ -220,70 +194,53 @@ __global__ __launch_bounds__(RW* CW* kWave) void mx_gemm_tiles_kernel(const MxAr
   // workgroup -> (row block, column block): an XCD's workgroups one behind the other, eight row blocks of a column block side by side
   const int total = a.m_blocks * a.n_blocks, per_xcd = (total + 7) / 8;
   const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per_xcd || id >= total) return;   // the whole workgroup
+  if (id >= total) return;   // the whole workgroup
   const int group = id / (8 * a.n_blocks), first = group * 8, rows_here = min(8, a.m_blocks - first), in = id - group * 8 * a.n_blocks;
   const int mb = first + in % rows_here, nb = in / rows_here;
-  const int m0 = mb * kRows, n0 = (nb * CW + wc) * (32 * TN);
-  const int k_tiles = a.k_tiles, k_groups = (k_tiles + 3) / 4, steps = k_tiles / KT;
-  const int s_begin = blockIdx.y * a.per_split, n_steps = min(a.per_split, steps - s_begin);
+  const int m0 = mb * kRows, tile0 = nb * kTiles, n0 = (nb * CW + wc) * (32 * TN);
+  const int k_tiles = a.k_tiles, rounds = k_tiles / 4;
+  const int r_begin = blockIdx.y * a.per_split, n_rounds = min(a.per_split, rounds - r_begin), n_steps = 4 * n_rounds;
 
-  const uint8_t* wptr[TN];
-  const uint32_t* wsptr[TN];
+  // what the wave fetches: XD kilobytes of rows of X, tiles WD wave .. of W, 64 rows' scales (the first waves), every fourth tile group's scales
+  const auto slot = [](int row, int c) { return BITS == kMx8 ? c ^ (row >> 1 & 7) : c ^ (row >> 2 & 3); };   // of piece c; and the piece of slot c
+  const uint8_t* const x0 = a.x + static_cast<int64_t>(m0) * a.ldx;
+  uint32_t x_off[XD];
 #pragma unroll
-  for (int tn = 0; tn < TN; ++tn) {
-    const int64_t tile = min(n0 / 16 + 2 * tn + (j >> 4), a.n_tiles - 1);
-    wptr[tn] = a.w + tile * k_tiles * 1024 + (16 * h + (j & 15)) * 16;
-    wsptr[tn] = a.ws + tile * k_groups * 64 + 16 * h + (j & 15);
+  for (int p = 0; p < XD; ++p) {
+    const int row = kRowsALoad * (XD * wave + p) + lane / kPieces;
+    x_off[p] = static_cast<uint32_t>(min(row, a.M - 1 - m0)) * static_cast<uint32_t>(a.ldx) + slot(row, lane % kPieces) * 16;
   }
-  struct WStep {
-    u32x4 w[TN][KK];
-    uint32_t s[TN][2];      // of the 512 k that the step lies in
-  };
-  auto load_w = [&](int s, WStep& d) {
-    const int kt = min(s_begin + s, steps - 1) * KT;
+  const uint8_t* w0[WD];
 #pragma unroll
-    for (int tn = 0; tn < TN; ++tn) {
+  for (int q = 0; q < WD; ++q) w0[q] = a.w + static_cast<int64_t>(min(tile0 + WD * wave + q, a.n_tiles - 1)) * k_tiles * 1024;
+  // a round's scales are kilobytes too: 64 rows of X or four tiles of W; which is which is a matter of addresses, as a branch in the loop
+  // would part it into pieces between which the compiler moves products; a load too many is the last one again
+  constexpr int kXItems = kXScales / 1024, kItems = kXItems + kTiles / 4, SD = (kItems + kWaves - 1) / kWaves;
+  const uint8_t* s0[SD];
+  uint32_t s_off[SD];
+  int s_step[SD], s_to[SD];
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
-        d.w[tn][kk] = *reinterpret_cast<const u32x4*>(wptr[tn] + static_cast<int64_t>(kt) * 1024 + kk * 512);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) d.s[tn][half] = wsptr[tn][(kt >> 2) * 64 + half * 32];
-    }
-  };
-  const uint8_t* xptr[XH];
-  int park_at[XH];
-#pragma unroll
-  for (int p = 0; p < XH; ++p) {
-    const int row = (p * kThreads + tid) >> 3, c = tid & 7;
-    xptr[p] = a.x + static_cast<int64_t>(min(m0 + row, a.M - 1)) * a.ldx + c * 16;
-    park_at[p] = row * 128 + (c ^ (row & 7)) * 16;
+  for (int q = 0; q < SD; ++q) {
+    const int item = min(SD * wave + q, kItems - 1);
+    const bool of_x = item < kXItems;
+    s0[q] = of_x ? a.xs + static_cast<int64_t>(m0) * a.ldxs : reinterpret_cast<const uint8_t*>(a.ws);
+    s_off[q] = of_x ? static_cast<uint32_t>(min(64 * item + lane, a.M - 1 - m0)) * static_cast<uint32_t>(a.ldxs)
+                    : static_cast<uint32_t>(min(tile0 + 4 * (item - kXItems) + (lane >> 4), a.n_tiles - 1) * rounds) * 256u + (lane & 15) * 16;
+    s_step[q] = of_x ? 16 : 256;
+    s_to[q] = item * 1024;
   }
-  const uint8_t* xsptr[XS];
+  // step s of this part; past its end the last step again, so that every step has as many loads
+  auto fetch_scales = [&](int s) {
+    const int round = r_begin + min(s, n_steps - 1) / 4;
 #pragma unroll
-  for (int p = 0; p < XS; ++p) xsptr[p] = a.xs + static_cast<int64_t>(min(m0 + min(p * kThreads + tid, kRows - 1), a.M - 1)) * a.ldxs;
-  struct XStep {
-    u32x4 x[XH];
-    uint32_t s[XS][KT];
+    for (int q = 0; q < SD; ++q) load_to_lds_16(s0[q] + static_cast<int64_t>(round) * s_step[q], s_off[q], lds_scales + (s / 4 & 1) * kScales + s_to[q]);
   };
-  auto load_x = [&](int s, XStep& d) {
-    const int64_t at = min(s_begin + s, steps - 1);
-#pragma unroll
-    for (int p = 0; p < XH; ++p) d.x[p] = *reinterpret_cast<const u32x4*>(xptr[p] + at * 128);
-#pragma unroll
-    for (int p = 0; p < XS; ++p)
-#pragma unroll
-      for (int q = 0; q < KT; ++q) d.s[p][q] = *reinterpret_cast<const uint32_t*>(xsptr[p] + at * 4 * KT + 4 * q);
-  };
-  auto park_x = [&](int stage, const XStep& d) {
-    unsigned char* to = lds + stage * kStage;
-#pragma unroll
-    for (int p = 0; p < XH; ++p) *reinterpret_cast<u32x4*>(to + park_at[p]) = d.x[p];
-#pragma unroll
-    for (int p = 0; p < XS; ++p)
-      if (p * kThreads + tid < kRows) {
-#pragma unroll
-        for (int q = 0; q < KT; ++q) *reinterpret_cast<uint32_t*>(to + kRows * 128 + (q * kRows + p * kThreads + tid) * 4) = d.s[p][q];
-      }
+  auto fetch = [&](int s, unsigned char* to, int i) {     // load i of the batch
+    const int64_t abs = 4 * r_begin + min(s, n_steps - 1);
+    if (i < XD)
+      load_to_lds_16(x0 + abs * kRowBytes, x_off[i], to + (XD * wave + i) * 1024);
+    else
+      load_to_lds_16(w0[i - XD] + abs * 1024, lane * 16, to + kXBytes + (WD * wave + i - XD) * 1024);
   };
 
   mx_f32x16 acc[MT][TN];
@@ -293,123 +250,210 @@ __global__ __launch_bounds__(RW* CW* kWave) void mx_gemm_tiles_kernel(const MxAr
     for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[t][tn][r] = 0.f;
-  const int row_at = (wr * 32 * MT + j);
-  auto multiply = [&](int s, int stage, const WStep& d) {
-    const unsigned char* from = lds + stage * kStage;
-    const int kt = (s_begin + s) * KT;
-    uint32_t xs[MT][KT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int q = 0; q < KT; ++q)
-        xs[t][q] = *reinterpret_cast<const uint32_t*>(from + kRows * 128 + (q * kRows + row_at + 32 * t) * 4) >> (8 * h);
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      int wscale[TN];
-#pragma unroll
-      for (int tn = 0; tn < TN; ++tn) wscale[tn] = static_cast<int>(d.s[tn][kk & 1] >> (8 * ((kt + kk / 2) & 3)));
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const unsigned char* row = from + (row_at + 32 * t) * 128;
-        mx_i32x8 xo;
-        if constexpr (BITS == kMx8)
-          xo = mx_operand8(*reinterpret_cast<const u32x4*>(row + ((4 * kk + h) ^ (j & 7)) * 16),
-                           *reinterpret_cast<const u32x4*>(row + ((4 * kk + 2 + h) ^ (j & 7)) * 16));
-        else
-          xo = mx_operand4(*reinterpret_cast<const u32x4*>(row + ((2 * kk + h) ^ (j & 7)) * 16));
-        const int xscale = static_cast<int>(xs[t][kk / 2]);
-#pragma unroll
-        for (int tn = 0; tn < TN; ++tn) {
-          if ((kk & 1) == 0)
-            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(d.w[tn][kk]), xo, acc[t][tn], 4, BITS == kMx8 ? 0 : 4, 0,
-                                                                         wscale[tn], 0, xscale);
-          else
-            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(d.w[tn][kk]), xo, acc[t][tn], 4, BITS == kMx8 ? 0 : 4, 0,
-                                                                         wscale[tn], 2, xscale);
-        }
-      }
+
+  // this lane's places in a stage: a piece of X row 32 (MT wr + t) + j is at x_at with bits exchanged; W
+  const int x_at = (wr * 32 * MT + j) * kRowBytes + slot(j, h) * 16;
+  const int w_at = kXBytes + (wc * 2 * TN + (j >> 4)) * 1024 + (16 * h + (j & 15)) * 16;
+  struct XOperand {      // registers of its own size: eight of which four are zeros would be eight registers across the loop
+    u32x4 part[BITS == kMx8 ? 2 : 1];
+    __device__ mx_i32x8 whole() const {
+      if constexpr (BITS == kMx8)
+        return mx_operand8(part[0], part[1]);
+      else
+        return mx_operand4(part[0]);
     }
   };
+  auto read_x = [&](const unsigned char* from, int kk, int t, int part) {
+    return *reinterpret_cast<const u32x4*>(from + (x_at ^ (BITS == kMx8 ? 64 * kk + 32 * part : 32 * kk)) + 32 * kRowBytes * t);
+  };
+  auto read_w = [&](const unsigned char* from, int kk, int tn) { return *reinterpret_cast<const u32x4*>(from + w_at + 2048 * tn + 512 * kk); };
+  u32x4 xs[MT];          // of a round: a row's sixteen bytes, turned so that this lane's blocks are bytes 0 and 2 of the step's word
+  uint32_t ws[TN][2];
+  auto read_scales = [&](int round) {
+    const unsigned char* sc = lds_scales + (round & 1) * kScales;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xs[t] = *reinterpret_cast<const u32x4*>(sc + (wr * 32 * MT + 32 * t + j) * 16) >> (8u * h);
+#pragma unroll
+    for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        ws[tn][half] = *reinterpret_cast<const uint32_t*>(sc + kXScales + (wc * 2 * TN + 2 * tn + (j >> 4)) * 256 + (16 * (2 * half + h) + (j & 15)) * 4);
+  };
+  XOperand xo[2];
+  u32x4 wo[2][TN];
+  constexpr int kFormat = BITS == kMx8 ? 0 : 4;
+  auto batch_landed = [] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * kBatch) : "memory"); };   // all but the youngest batches
 
-  WStep wring[PD];
-  XStep xnext;
-  load_x(0, xnext);
 #pragma unroll
-  for (int u = 0; u < PD; ++u) load_w(u, wring[u]);
-  park_x(0, xnext);
-  load_x(1, xnext);
-  __syncthreads();
-  for (int s0 = 0; s0 < n_steps; s0 += PD) {
+  for (int s = 0; s < STAGES - 1; ++s) {
+    if (s % 4 == 0) fetch_scales(s);
 #pragma unroll
-    for (int u = 0; u < PD; ++u) {
-      const int s = s0 + u;
-      if (s < n_steps) {                          // the same in the whole workgroup
-        park_x((u + 1) & 1, xnext);               // everybody is past the step that read that stage
-        load_x(s + 2, xnext);
-        multiply(s, u & 1, wring[u]);
-        load_w(s + PD, wring[u]);
-        __syncthreads();
-      }
-    }
+    for (int i = 0; i < kBatch; ++i) fetch(s, lds + s * kStage, i);
   }
+  batch_landed();
+  __syncthreads();
+  read_scales(0);
+#pragma unroll
+  for (int part = 0; part < (BITS == kMx8 ? 2 : 1); ++part) xo[0].part[part] = read_x(lds, 0, 0, part);
+#pragma unroll
+  for (int tn = 0; tn < TN; ++tn) wo[0][tn] = read_w(lds, 0, tn);
+  unsigned char *now = lds, *last = lds + (STAGES - 1) * kStage;     // the stage of this step; where the batch goes
+  for (int r = 0; r < n_rounds; ++r) {
+    auto step = [&](auto uc) {
+      constexpr int u = decltype(uc)::value;
+      const int s = 4 * r + u;
+      unsigned char* next = now == lds + (STAGES - 1) * kStage ? lds : now + kStage;
+      if constexpr (u == (9 - STAGES) % 4) fetch_scales(s + STAGES - 1);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int kk = g / MT, t = g % MT;
+        if (g == kGroups - 1) {
+          batch_landed();
+          __syncthreads();
+        }
+        const unsigned char* from = g == kGroups - 1 ? next : now;
+        const int gn = (g + 1) % kGroups;
+        const int xscale = static_cast<int>(xs[t][u]);
+        const mx_i32x8 x = xo[g & 1].whole();
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn) {
+          // in front of every product a piece of the operands of the group behind, and a load of the batch here and there
+          constexpr int kParts = BITS == kMx8 ? 2 : 1;
+#pragma unroll
+          for (int part = 0; part < kParts; ++part)
+            if (TN == 1 || tn == part) xo[(g + 1) & 1].part[part] = read_x(from, gn / MT, gn % MT, part);
+          if (t == MT - 1) wo[(kk + 1) & 1][tn] = read_w(from, (kk + 1) & 1, tn);
+          constexpr int kSlots = (kGroups - 1) * TN;
+          const int slot_at = g * TN + tn;
+          if (slot_at < kSlots) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+              if (i * kSlots / kBatch == slot_at) fetch(s + STAGES - 1, last, i);
+          }
+          // the byte of W's scale word is the step inside the round, that of X's the half
+          if (kk == 0)
+            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[0][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(ws[tn][0]), 0,
+                                                                         xscale);
+          else
+            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[1][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(ws[tn][1]), 2,
+                                                                         xscale);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if constexpr (u == 3) read_scales(r + 1);
+      last = now;
+      now = next;
+    };
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+    step(std::integral_constant<int, 2>{});
+    step(std::integral_constant<int, 3>{});
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the batches past the end: nothing may land in what follows
+  __syncthreads();
 
-  // acc[t][tn][r] = C[m0 + 32 (MT wr + t) + j][n0 + 32 tn + 8 (r / 4) + 4 h + r % 4]
+  // acc[t][tn][r] = C[m0 + 32 (MT wr + t) + j][n0 + 32 tn + 8 (r / 4) + 4 h + r % 4].  Stored as they are, a lane's four columns are scraps of 4
+  // to 16 bytes of a row; they go through a part of LDS that belongs to the wave and leave as whole runs of a row, 16 bytes a lane.
+  constexpr int kRun = kGate ? (EPI == kMxGate8 ? 16 * TN : 8 * TN) : (EPI == kMxBf16 ? 64 * TN : 128);   // bytes of a row
+  constexpr int kPitch = kRun + 16, kLanes = kRun / 16, kRowsAPass = kWave / kLanes;
+  static_assert(kWaves * 32 * kPitch <= STAGES * kStage, "the wave's part of the stages");
+  unsigned char* const mine = lds + wave * (32 * kPitch);
+  auto settle = [] {     // what the wave's lanes wrote is there for its other lanes
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  auto leave = [&](int row0, unsigned char* out, int64_t pitch) {     // out: the run's place in row row0
+    settle();
+#pragma unroll
+    for (int i = 0; i < (32 + kRowsAPass - 1) / kRowsAPass; ++i) {
+      const int rr = kRowsAPass * i + lane / kLanes, piece = lane % kLanes;
+      if (rr < 32 && row0 + rr < a.M)
+        *reinterpret_cast<u32x4*>(out + rr * pitch + piece * 16) = *reinterpret_cast<const u32x4*>(mine + rr * kPitch + piece * 16);
+    }
+    settle();
+  };
   if constexpr (kGate) {
     constexpr int kBits = EPI == kMxGate8 ? kMx8 : kMx4;
-    if (n0 / 16 >= a.n_tiles) return;             // (whole blocks: the columns are a multiple of 512)
+    if (n0 / 16 >= a.n_tiles) return;             // whole blocks: the columns are a multiple of 512
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      float4 v[TN][2];
-      uint32_t most = 0;
+      const int row0 = m0 + 32 * (MT * wr + t);
 #pragma unroll
-      for (int tn = 0; tn < TN; ++tn)
+      for (int b = 0; b < TN / 2; ++b) {          // blocks of 32 results
+        float4 v[2][2];
+        uint32_t most = 0;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          v[tn][q] = float4{mx_silu_mul(acc[t][tn][4 * q], acc[t][tn][4 * q + 8]), mx_silu_mul(acc[t][tn][4 * q + 1], acc[t][tn][4 * q + 9]),
-                            mx_silu_mul(acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 10]), mx_silu_mul(acc[t][tn][4 * q + 3], acc[t][tn][4 * q + 11])};
-          most = max(most, mx_max4(v[tn][q]));
-        }
-      const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
-      const uint32_t code = mx_code<kBits>(max(both[0], both[1]));
-      const int row = m0 + 32 * (MT * wr + t) + j;
-      if (row < a.M) {
-        uint8_t* o = static_cast<uint8_t*>(a.out) + row * a.ldo;
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const mx_f32x16& c = acc[t][2 * b + p];
+            v[p][q] = float4{mx_silu_mul(c[4 * q], c[4 * q + 8]), mx_silu_mul(c[4 * q + 1], c[4 * q + 9]), mx_silu_mul(c[4 * q + 2], c[4 * q + 10]),
+                             mx_silu_mul(c[4 * q + 3], c[4 * q + 11])};
+            most = max(most, mx_max4(v[p][q]));
+          }
+        const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+        const uint32_t code = mx_code<kBits>(max(both[0], both[1]));
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) mx_store4<kBits>(mine + j * kPitch, 32 * b + 16 * p + 8 * q + 4 * h, mx_pack4<kBits>(v[p][q], code));
+        if (h == 0 && row0 + j < a.M) a.out_scales[(row0 + j) * a.ldos + n0 / 64 + b] = static_cast<uint8_t>(code);
+      }
+      leave(row0, static_cast<uint8_t*>(a.out) + row0 * a.ldo + n0 / 2 * kBits / 8, a.ldo);
+    }
+  } else {
+    const bool whole = a.vec && n0 + 32 * TN <= a.N;      // the same in all lanes
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const int row0 = m0 + 32 * (MT * wr + t);
+      if (!whole) {
 #pragma unroll
         for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) mx_store4<kBits>(o, n0 / 2 + 16 * tn + 8 * q + 4 * h, mx_pack4<kBits>(v[tn][q], code));
-        if (h == 0) a.out_scales[row * a.ldos + n0 / 64] = static_cast<uint8_t>(code);
+          for (int q = 0; q < 4; ++q)
+            mx_store_sums<EPI>(a, blockIdx.y, row0 + j, n0 + 32 * tn + 8 * q + 4 * h,
+                               mx_f32x4{acc[t][tn][4 * q], acc[t][tn][4 * q + 1], acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3]});
+      } else if constexpr (EPI == kMxBf16) {
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint2*>(mine + j * kPitch + (32 * tn + 8 * q + 4 * h) * 2) =
+                uint2{pack_bf16x2(acc[t][tn][4 * q], acc[t][tn][4 * q + 1]), pack_bf16x2(acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3])};
+        leave(row0, reinterpret_cast<unsigned char*>(static_cast<bf16*>(a.out) + row0 * a.ldo + n0), a.ldo * 2);
+      } else {
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<mx_f32x4*>(mine + j * kPitch + (8 * q + 4 * h) * 4) =
+                mx_f32x4{acc[t][tn][4 * q], acc[t][tn][4 * q + 1], acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3]};
+          leave(row0, reinterpret_cast<unsigned char*>(static_cast<float*>(a.out) + blockIdx.y * a.split_stride + row0 * a.ldo + n0 + 32 * tn), a.ldo * 4);
+        }
       }
     }
-  } else {
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int tn = 0; tn < TN; ++tn)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          mx_store_sums<EPI>(a, blockIdx.y, m0 + 32 * (MT * wr + t) + j, n0 + 32 * tn + 8 * q + 4 * h,
-                             mx_f32x4{acc[t][tn][4 * q], acc[t][tn][4 * q + 1], acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3]});
   }
 }
 
 // ---- launches
 
-template <int BITS, int EPI, int RT, int CT, int WAVES, int U>
+template <int BITS, int EPI, int CT, int WAVES>
 int mx_rows_launch(const MxArgs& a, int splits, hipStream_t s) {
-  mx_gemm_rows_kernel<BITS, RT, CT, WAVES, U, EPI><<<dim3((a.n_tiles + CT - 1) / CT, splits), WAVES * kWave, 0, s>>>(a);
+  mx_gemm_rows_kernel<BITS, CT, WAVES, EPI><<<dim3((a.n_tiles + CT - 1) / CT, splits), WAVES * kWave, 0, s>>>(a);
   return launch_status();
 }
 
-template <int BITS, int EPI, int MT, int TN, int RW, int CW, int PD>
+template <int BITS, int EPI, int MT, int TN, int RW, int CW, int STAGES, int WAVES_A_SIMD>
 int mx_tiles_launch(MxArgs a, int splits, hipStream_t s) {
   static OnceADevice asked;
-  constexpr int kRows = 32 * MT * RW;
-  constexpr size_t kLds = 2 * kRows * (128 + (BITS == kMx8 ? 4 : 8));
-  const auto kernel = mx_gemm_tiles_kernel<BITS, MT, TN, RW, CW, PD, EPI>;
+  constexpr int kRows = 32 * MT * RW, kTiles = 2 * TN * CW;
+  constexpr size_t kLds = STAGES * (kRows * 16 * BITS + kTiles * 1024) + 2 * ((kRows < 64 ? 64 : kRows) * 16 + kTiles * 256);
+  static_assert(kLds <= 160 * 1024, "what a compute unit has");
+  const auto kernel = mx_gemm_tiles_kernel<BITS, MT, TN, RW, CW, STAGES, WAVES_A_SIMD, EPI>;
   if (const int e = ask_lds(asked, kLds, {reinterpret_cast<const void*>(kernel)})) return e;
   a.m_blocks = (a.M + kRows - 1) / kRows;
-  a.n_blocks = (a.n_tiles + 2 * TN * CW - 1) / (2 * TN * CW);
+  a.n_blocks = (a.n_tiles + kTiles - 1) / kTiles;
   const int per_xcd = (a.m_blocks * a.n_blocks + 7) / 8;
   kernel<<<dim3(8 * per_xcd, splits), RW * CW * kWave, kLds, s>>>(a);
   return launch_status();
@@ -419,13 +463,14 @@ template <int BITS, int EPI>
 int mx_launch(int variant, const MxArgs& a, int splits, hipStream_t s) {
   constexpr bool kGate = EPI == kMxGate8 || EPI == kMxGate4;
   switch (variant) {
-    case 0: return mx_rows_launch<BITS, EPI, 1, kGate ? 4 : 2, 8, 2>(a, splits, s);
-    case 1: return mx_rows_launch<BITS, EPI, 2, kGate ? 4 : 2, 8, 1>(a, splits, s);
-    case 2: return mx_rows_launch<BITS, EPI, 4, kGate ? 4 : 2, 4, 1>(a, splits, s);
-    case 3: return mx_tiles_launch<BITS, EPI, 1, 2, 2, 2, 2>(a, splits, s);
-    case 4: return mx_tiles_launch<BITS, EPI, 2, 2, 2, 2, 2>(a, splits, s);
-    case 5: return mx_tiles_launch<BITS, EPI, 4, 2, 1, 4, 2>(a, splits, s);
-    case 6: return mx_tiles_launch<BITS, EPI, 4, 2, 2, 4, 2>(a, splits, s);
+    case 0: if constexpr (!kGate) return mx_rows_launch<BITS, EPI, 2, 4>(a, splits, s); else break;
+    case 1: if constexpr (!kGate) return mx_rows_launch<BITS, EPI, 1, 8>(a, splits, s); else break;
+    case 2: if constexpr (!kGate) return mx_tiles_launch<BITS, EPI, 1, 1, 1, 2, 8, 1>(a, splits, s); else break;
+    case 3: return mx_tiles_launch<BITS, EPI, 1, 2, 2, 2, 8, 1>(a, splits, s);
+    case 4: return mx_tiles_launch<BITS, EPI, 2, 2, 2, 2, 3, 2>(a, splits, s);
+    case 5: return mx_tiles_launch<BITS, EPI, 2, 2, 2, 4, BITS == kMx8 ? 4 : 5, 2>(a, splits, s);
+    case 6: return mx_tiles_launch<BITS, EPI, 4, 2, 2, 4, BITS == kMx8 ? 3 : 4, 2>(a, splits, s);
+    case 7: if constexpr (!kGate) return mx_tiles_launch<BITS, EPI, 2, 3, 2, 2, 5, 1>(a, splits, s); else break;
   }
   return static_cast<int>(hipErrorInvalidValue);
 }

@@ -1,7 +1,7 @@
 // Rows to microscaled rows and back: quantisation, the numbers that elements stand for, and the residual's addition with
 // the root-mean-square norm whose rows go straight into blocks.
 //
-// A microscaled row is padded with zeros to a multiple of 256 numbers (`padded`), so that the products behind it walk whole
+// A microscaled row is padded with zeros to a multiple of 512 numbers (`padded`), so that the products behind it walk whole
 // steps; every byte of it is written here.
 #include "mx.h"
 

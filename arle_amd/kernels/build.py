@@ -61,6 +61,8 @@ SOURCES = {
 HEADERS = ("common.h", "once_a_device.h", "attention_static.h", "attention_args.h", "attention_stream.h", "attention_portions.h",
            "attention_portions_dma.h", "lds_loads.h", "attention_softcap_portions.h", "addend.h", "chunks.h", "lane_sums.h", "scaled_rows.h")
 # headers that only some sources include: they count for those alone, so that a change compiles no other library again
+# (the same with flags: "source" keeps a basic block in the order in which it is written, into which a loop's reads and products are woven by hand)
+OWN_FLAGS = {"mx_gemm": ["-mllvm", "-pre-RA-sched=source"]}
 OWN_HEADERS = {"mx_rows": ("mx.h",), "mx_gemm": ("mx.h",)}
 HOST_LIBS = ("host",)   # plain C++: page pool, block tables, step packing
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared"]
@@ -148,7 +150,7 @@ def source_hash(name: str) -> str:
     for fname in ((SOURCES[name],) if host else (SOURCES[name], *HEADERS, *OWN_HEADERS.get(name, ()))):
         with open(os.path.join(CSRC_DIR, fname), "rb") as fh:
             h.update(fh.read())
-    h.update(" ".join(HOST_FLAGS if host else HIPCC_FLAGS).encode())
+    h.update(" ".join([*(HOST_FLAGS if host else HIPCC_FLAGS), *OWN_FLAGS.get(name, ())]).encode())
     return h.hexdigest()
 
 
@@ -172,7 +174,7 @@ def build(name: str) -> str:
         cmd = [find_host_compiler(), *HOST_FLAGS, src, "-o", tmp]
         _say(f"compiling {SOURCES[name]} for the host ...")
     else:
-        cmd = [find_hipcc(), *HIPCC_FLAGS, f"-I{CSRC_DIR}", src, "-o", tmp]
+        cmd = [find_hipcc(), *HIPCC_FLAGS, *OWN_FLAGS.get(name, ()), f"-I{CSRC_DIR}", src, "-o", tmp]
         _say(f"compiling {SOURCES[name]} for {OFFLOAD_ARCH} ...")
     t0 = time.time()
     env = dict(os.environ)

@@ -10,108 +10,152 @@ path.
 """
 from __future__ import annotations
 
-import dataclasses
-import math
+import collections
+import functools
 
 import torch
 
 from . import lib, ops
-from .ops import BF16, F32, ShapeError, _code, _i32, _need, _ptr, _rows, _stream
+from .ops import _CODES, F32, ShapeError, _ptr
 
 BLOCK = 32
-PAD = 256                # a row's numbers are padded with zeros to a multiple of this, for products that walk whole steps
+PAD = 512                # a row's numbers are padded with zeros to a multiple of this, for products that walk whole steps
 TILE = 128               # k of an operand tile
+MAX_K = 2**22            # numbers of a row: 256 rows of elements are within 32 bits of offsets
+MAX_WEIGHT = 2**35       # numbers of a weight: its scales are
 MAX_WIDTH = 16384        # of a norm's rows, which the kernel keeps in registers
 BITS = {"mxfp8": 8, "mxfp4": 4}
-_GRID_MAX = 2**31 - 1
+_ELEMENTS = {"mxfp8": torch.float8_e4m3fn, "mxfp4": torch.uint8}
+_SCALES = torch.float8_e8m0fnu
 
 
-def _here(*tensors) -> None:
-    """All on one GPU, the current one: the stream that a kernel runs on is the current device's."""
+# The checks below are plain `if`s whose message is made only where it is raised, and rows and weights are checked where they are
+# made, not at every call: with eagerly made messages and checks at every use a product of a few rows cost the host 14 us, so 6.
+
+
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _here(*tensors) -> int:
+    """The current device, the one whose stream a kernel runs on and that all of the tensors have to be on."""
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
+        if t is not None and not t.is_cuda:
             raise ShapeError("arle_amd kernels run on the GPU only; got a CPU tensor")
-        if t.device.index != torch.cuda.current_device():
-            raise ShapeError(f"tensor on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    device = _current()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ShapeError(f"tensor on {t.device}, the current device is cuda:{device}")
+    return device
+
+
+def _same_device(held: int) -> int:
+    """The current device, which has to be the one that rows and weights are held on."""
+    device = _current()
+    if held != device:
+        raise ShapeError(f"rows or weights on cuda:{held}, the current device is cuda:{device}")
+    return device
+
+
+_functions: dict = {}
+
+
+def _call(name: str, *args) -> None:
+    """lib.call with the function found once."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = lib.function(name)
+    status = fn(*args)
+    if status:
+        raise lib.KernelError(f"{name} failed with HIP error {status}")
+
+
+def _stream(device: int) -> int:
+    return ops._raw_stream(device) if ops._raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _bits(form: str) -> int:
-    _need(form in BITS, f"unknown form {form!r} (known: {', '.join(BITS)})")
-    return BITS[form]
+    bits = BITS.get(form)
+    if bits is None:
+        raise ShapeError(f"unknown form {form!r} (known: {', '.join(BITS)})")
+    return bits
 
 
 def padded_width(width: int) -> int:
     return -(-width // PAD) * PAD
 
 
-@dataclasses.dataclass(frozen=True)
-class MXRows:
-    """Rows in blocks.  elements uint8: [T, padded] (mxfp8) or [T, padded / 2] (mxfp4, the number with the lower index in the lower
-    half of a byte); scales uint8 [T, padded / 32]; zeros from `width` to `padded`, the next multiple of 256."""
-    elements: torch.Tensor
-    scales: torch.Tensor
-    width: int
-    form: str
+_Rows = collections.namedtuple("_Rows", "elements scales width form rows padded bits device")
 
-    @property
-    def rows(self) -> int:
-        return self.elements.shape[0]
 
-    @property
-    def padded(self) -> int:
-        return padded_width(self.width)
+class MXRows(_Rows):
+    """Rows in blocks, MXRows(elements, scales, width, form).  elements: float8_e4m3fn [T, padded] (mxfp8) or uint8 [T, padded / 2] (mxfp4, the number
+    with the lower index in the lower half of a byte); scales float8_e8m0fnu [T, padded / 32]; zeros (codes of 0) from `width` to `padded`, the next
+    multiple of 512.  Views whose rows lie apart are fine where rows start at multiples of 16 bytes."""
+    __slots__ = ()
+
+    def __new__(cls, elements: torch.Tensor, scales: torch.Tensor, width: int, form: str):
+        bits = _bits(form)
+        device = _here(elements, scales)
+        if not 1 <= width <= MAX_K:
+            raise ShapeError(f"rows have 1 to {MAX_K} columns, got {width}")
+        padded = padded_width(width)
+        e, s = elements, scales
+        if not (e.dtype == _ELEMENTS[form] and e.dim() == 2 and e.shape[1] == padded * bits // 8 and s.dtype == _SCALES
+                and tuple(s.shape) == (e.shape[0], padded // BLOCK)):
+            raise ShapeError(f"{form} rows of {width} are {_ELEMENTS[form]} [T, {padded * bits // 8}] with scales {_SCALES} [T, {padded // BLOCK}], got "
+                             f"{e.dtype} {tuple(e.shape)} with {s.dtype} {tuple(s.shape)}")
+        if e.stride(1) != 1 or s.stride(1) != 1 or e.data_ptr() % 16 or s.data_ptr() % 16 or (e.shape[0] > 1 and (e.stride(0) % 16 or s.stride(0) % 16 or e.stride(0) > 2 * MAX_K)):
+            raise ShapeError("rows of elements and scales must lie together and start at multiples of 16 bytes")
+        return tuple.__new__(cls, (e, s, int(width), form, e.shape[0], padded, bits, device))
+
+    def part(self, start: int, stop: int) -> "MXRows":
+        """Rows start .. stop - 1, a view."""
+        return MXRows(self.elements[start:stop], self.scales[start:stop], self.width, self.form)
 
     def elements_e4m3(self) -> torch.Tensor:
-        """The elements of "mxfp8" rows as torch's type, a view."""
-        _need(self.form == "mxfp8", f"{self.form} elements are no e4m3")
-        return self.elements[:, :self.width].view(torch.float8_e4m3fn)
+        """The elements of "mxfp8" rows without the padding, a view [T, width]."""
+        if self.bits != 8:
+            raise ShapeError(f"{self.form} elements are no e4m3")
+        return self.elements if self.width == self.padded else self.elements[:, :self.width]
 
     def scales_e8m0(self) -> torch.Tensor:
-        """The scales as torch's type of bare exponents, a view [T, ceil(width / 32)]."""
-        return self.scales[:, :-(-self.width // BLOCK)].view(torch.float8_e8m0fnu)
-
-    def __getitem__(self, rows: slice) -> "MXRows":
-        _need(isinstance(rows, slice), "MXRows take a slice of rows")
-        return MXRows(self.elements[rows], self.scales[rows], self.width, self.form)
+        """The scales without the padding, a view [T, ceil(width / 32)]."""
+        return self.scales if self.width == self.padded else self.scales[:, :-(-self.width // BLOCK)]
 
 
-def _empty_rows(rows: int, width: int, form: str, device) -> MXRows:
-    padded = padded_width(width)
-    return MXRows(torch.empty((rows, padded * BITS[form] // 8), dtype=torch.uint8, device=device),
-                  torch.empty((rows, padded // BLOCK), dtype=torch.uint8, device=device), width, form)
+_new = tuple.__new__
+_empty = torch.empty
 
 
-def _check_rows(x: MXRows, name: str = "x") -> None:
-    """The kernels read 16 bytes of elements and words of scales at a time."""
-    _need(type(x) is MXRows, f"{name} must be MXRows (see quantize), got {type(x).__name__}")
-    bits = _bits(x.form)
-    _here(x.elements, x.scales)
-    e, s = x.elements, x.scales
-    _need(x.width > 0, f"{name}: no columns")
-    _need(e.dtype == torch.uint8 and e.dim() == 2 and e.shape[1] == x.padded * bits // 8 and s.dtype == torch.uint8
-          and tuple(s.shape) == (e.shape[0], x.padded // BLOCK),
-          f"{name}: {x.form} rows of {x.width} are uint8 [T, {x.padded * bits // 8}] and [T, {x.padded // BLOCK}]")
-    _need(e.shape[0] <= 1 or (e.stride(0) % 16 == 0 and s.stride(0) % 4 == 0), f"{name}: rows must be 16 bytes apart, scales 4")
-    _need(e.stride(1) == 1 and s.stride(1) == 1 and e.data_ptr() % 16 == 0 and s.data_ptr() % 4 == 0,
-          f"{name}: elements must start at 16 bytes, scales at 4, both with contiguous rows")
+def _new_rows(rows: int, width: int, form: str, bits: int, device: int) -> MXRows:
+    padded, on = -(-width // PAD) * PAD, _DEVICES.get(device) or _device(device)
+    return _new(MXRows, (_empty(rows, padded * bits // 8, dtype=_ELEMENTS[form], device=on), _empty(rows, padded // BLOCK, dtype=_SCALES, device=on),
+                         width, form, rows, padded, bits, device))
+
+
+_DEVICES: dict = {}
+
+
+def _device(index: int) -> torch.device:
+    return _DEVICES.setdefault(index, torch.device("cuda", index))
 
 
 def rows_from_codes(elements: torch.Tensor, scales: torch.Tensor, width: int, form: str) -> MXRows:
     """Rows from codes that exist already: elements uint8 [T, at least width], a code a byte in both forms; scales uint8 [T, ceil(width / 32)]."""
     bits = _bits(form)
     _here(elements, scales)
-    _need(elements.dtype == torch.uint8 and elements.dim() == 2 and scales.dtype == torch.uint8 and scales.dim() == 2, "codes are uint8 [T, ...]")
-    T = elements.shape[0]
     blocks = -(-width // BLOCK)
-    _need(width > 0 and elements.shape[1] >= width and tuple(scales.shape) == (T, blocks), f"codes of rows of {width} are [T, {width}] and [T, {blocks}]")
+    if not (elements.dtype == torch.uint8 and elements.dim() == 2 and scales.dtype == torch.uint8 and width > 0 and elements.shape[1] >= width
+            and tuple(scales.shape) == (elements.shape[0], blocks)):
+        raise ShapeError(f"codes of rows of {width} are uint8 [T, {width}] and [T, {blocks}], got {elements.dtype} {tuple(elements.shape)} and "
+                         f"{scales.dtype} {tuple(scales.shape)}")
     padded = padded_width(width)
     e = torch.nn.functional.pad(elements[:, :width], (0, padded - width))
     if bits == 4:
-        _need(T == 0 or int(e.max()) < 16, "a code of 4 bits is under 16")
+        if e.numel() and int(e.max()) > 15:
+            raise ShapeError("a code of 4 bits is under 16")
         e = e[:, 0::2] | (e[:, 1::2] << 4)
-    return MXRows(e.contiguous(), torch.nn.functional.pad(scales, (0, padded // BLOCK - blocks)).contiguous(), width, form)
+    return MXRows(e.contiguous().view(_ELEMENTS[form]), torch.nn.functional.pad(scales, (0, padded // BLOCK - blocks)).contiguous().view(_SCALES), width, form)
 
 
 # ----------------------------------------------------------------------- rows
@@ -119,30 +163,36 @@ def rows_from_codes(elements: torch.Tensor, scales: torch.Tensor, width: int, fo
 
 def quantize(x: torch.Tensor, form: str = "mxfp8") -> MXRows:
     """x [T, K] float32 or bfloat16 in blocks of 32 along K."""
-    bits = _bits(form)
-    _here(x)
-    _rows(x, "x")
+    bits = BITS.get(form) or _bits(form)
+    device = x.get_device()
+    if device < 0 or device != _current():
+        _here(x)
+    code = _CODES.get(x.dtype)
+    if code is None or x.dim() != 2:
+        raise ShapeError(f"quantize takes float32 or bfloat16 [T, K], got {x.dtype} {tuple(x.shape)}")
     T, K = x.shape
-    _need(K > 0, "quantize: no columns")
-    _need(T <= _GRID_MAX and padded_width(K) < 2**27, "quantize: too large for one launch")
-    out = _empty_rows(T, K, form, x.device)
-    if T == 0:
-        return out
-    size = x.element_size()
-    aligned = K % 8 == 0 and x.data_ptr() % (4 * size) == 0 and x.stride(0) % 4 == 0
-    lib.call("arle_mx_quantize", x.data_ptr(), _code(x), x.stride(0), out.elements.data_ptr(), out.scales.data_ptr(), bits, T, K, out.padded,
-             int(aligned), _stream())
+    stride, step = x.stride()
+    if K < 1 or (step != 1 and K > 1) or K > MAX_K:
+        raise ShapeError(f"quantize takes rows of 1 to {MAX_K} numbers that lie together, got {tuple(x.shape)} with strides {tuple(x.stride())}")
+    out = _new_rows(T, K, form, bits, device)
+    if T:
+        at = x.data_ptr()
+        aligned = K % 8 == 0 and stride % 4 == 0 and at % (16 if code == F32 else 8) == 0
+        _call("arle_mx_quantize", at, code, stride, out[0].data_ptr(), out[1].data_ptr(), bits, T, K, out[5], aligned, _stream(device))
     return out
 
 
 def values(x: MXRows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The numbers that the elements stand for, [T, width] in float32 (exact) or bfloat16 (exact but for numbers under its smallest normal one)."""
-    _check_rows(x)
-    _need(dtype in (torch.float32, torch.bfloat16), "values come in float32 or bfloat16")
-    out = torch.empty((x.rows, x.width), dtype=dtype, device=x.elements.device)
+    if type(x) is not MXRows:
+        raise ShapeError(f"values takes MXRows (see quantize), got {type(x).__name__}")
+    device = _same_device(x.device)
+    if dtype not in _CODES:
+        raise ShapeError("values come in float32 or bfloat16")
+    out = torch.empty((x.rows, x.width), dtype=dtype, device=_device(device))
     if x.rows:
-        lib.call("arle_mx_values", x.elements.data_ptr(), x.elements.stride(0), x.scales.data_ptr(), x.scales.stride(0), BITS[x.form],
-                 out.data_ptr(), _code(out), x.rows, x.width, _stream())
+        _call("arle_mx_values", x.elements.data_ptr(), x.elements.stride(0), x.scales.data_ptr(), x.scales.stride(0), x.bits, out.data_ptr(),
+                 _CODES[dtype], x.rows, x.width, _stream(device))
     return out
 
 
@@ -152,44 +202,67 @@ def add_rmsnorm(residual: torch.Tensor, delta: torch.Tensor | None, weight: torc
 
     delta is None, [T, H], or a stack [S, T, H] of partial sums that are added in the order of the stack, as for ops.add_rmsnorm;
     rows (int32): the rows of the residual that are wanted, the last time it is read."""
-    bits = _bits(form)
-    _here(residual, delta, weight, rows)
-    _need(residual.dtype == torch.float32 and residual.dim() == 2 and residual.is_contiguous(), "residual must be contiguous float32 [T, H]")
-    T, width = residual.shape
-    _need(0 < width <= MAX_WIDTH, f"a norm's rows have 1 to {MAX_WIDTH} columns, got {width}")
-    n_delta, delta_code = 0, F32
+    bits = BITS.get(form) or _bits(form)
+    device = residual.get_device()
+    if (device < 0 or device != _current() or weight.get_device() != device or (delta is not None and delta.get_device() != device)
+            or (rows is not None and rows.get_device() != device)):
+        _here(residual, delta, weight, rows)
+    shape = residual.shape
+    if residual.dtype != torch.float32 or len(shape) != 2 or not residual.is_contiguous():
+        raise ShapeError("residual must be contiguous float32 [T, H]")
+    T, width = shape
+    if not 0 < width <= MAX_WIDTH:
+        raise ShapeError(f"a norm's rows have 1 to {MAX_WIDTH} columns, got {width}")
+    at, w_at, w_code = residual.data_ptr(), weight.data_ptr(), _CODES.get(weight.dtype)
+    if weight.dim() != 1 or weight.numel() != width or w_code is None or not weight.is_contiguous():
+        raise ShapeError(f"norm weight must be float32 or bfloat16 [{width}]")
+    aligned = width % 4 == 0 and at % 16 == 0 and w_at % (16 if w_code == F32 else 8) == 0
+    n_delta = delta_at = delta_code = 0
     if delta is not None:
-        _need(delta.dim() in (2, 3) and tuple(delta.shape[-2:]) == (T, width) and delta.is_contiguous() and delta.dtype in ops._CODES
-              and (delta.dim() == 2 or delta.shape[0] >= 1), "delta must match the residual ([T, H] or a stack [S, T, H])")
-        n_delta, delta_code = (delta.shape[0] if delta.dim() == 3 else 1), _code(delta)
-    _need(weight.shape == (width,) and weight.is_contiguous(), "norm weight must be [width]")
+        n_delta, of, delta_code = 1, delta.shape, _CODES.get(delta.dtype)
+        if len(of) == 3:
+            n_delta, of = of[0], of[1:]
+        if of != shape or delta_code is None or n_delta < 1 or not delta.is_contiguous():
+            raise ShapeError("delta must match the residual ([T, H] or a stack [S, T, H]) in float32 or bfloat16")
+        delta_at = delta.data_ptr()
+        aligned = aligned and delta_at % (16 if delta_code == F32 else 8) == 0
     n_rows = T
     if rows is not None:
-        _i32(rows, "rows")
+        if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
+            raise ShapeError("rows must be int32 1-D")
         n_rows = rows.numel()
-    out = _empty_rows(n_rows, width, form, residual.device)
-    if n_rows == 0:
-        return out
-    ops_of = [t for t in (residual, delta, weight) if t is not None]
-    aligned = width % 4 == 0 and all(t.data_ptr() % (4 * t.element_size()) == 0 for t in ops_of)
-    lib.call("arle_mx_add_rmsnorm", residual.data_ptr(), _ptr(delta), n_delta, residual.numel(), delta_code, weight.data_ptr(), _code(weight),
-             out.elements.data_ptr(), out.scales.data_ptr(), bits, _ptr(rows), n_rows, width, out.padded, int(aligned), float(eps), _stream())
+    out = _new_rows(n_rows, width, form, bits, device)
+    if n_rows:
+        _call("arle_mx_add_rmsnorm", at, delta_at, n_delta, T * width, delta_code, w_at, w_code, out[0].data_ptr(), out[1].data_ptr(), bits,
+              _ptr(rows), n_rows, width, out[5], aligned, eps, _stream(device))
     return out
 
 
 # ------------------------------------------------------------------- products
 
 
-@dataclasses.dataclass(frozen=True)
-class MXWeight:
-    """A weight [n, k] in 4 bits, laid out for the products.  tiles uint8 [tiles of 16 rows, tiles of 128 k, 64, 16], scales uint8
+_Weight = collections.namedtuple("_Weight", "tiles scales n k gated n_tiles k_tiles device")
+
+
+class MXWeight(_Weight):
+    """A weight [n, k] in 4 bits, laid out for the products (see lay_weight).  tiles uint8 [tiles of 16 rows, tiles of 128 k, 64, 16], scales uint8
     [tiles of 16 rows, groups of 512 k, 64, 4].  gated: n = 2 * ff rows, the gate's and then the up's, held in turns of 16 with both
-    halves padded with zeros to a multiple of 256."""
-    tiles: torch.Tensor
-    scales: torch.Tensor
-    n: int
-    k: int
-    gated: bool = False
+    halves padded with zeros to a multiple of 512."""
+    __slots__ = ()
+
+    def __new__(cls, tiles: torch.Tensor, scales: torch.Tensor, n: int, k: int, gated: bool = False):
+        device = _here(tiles, scales)
+        if n < 1 or k < 1 or (gated and n % 2):
+            raise ShapeError(f"a weight of {n} rows of {k} ({'gated' if gated else 'plain'})")
+        if k > MAX_K or n * k > MAX_WEIGHT:
+            raise ShapeError(f"a weight has up to {MAX_K} columns and {MAX_WEIGHT} numbers, got [{n}, {k}]")
+        k_tiles = padded_width(k) // TILE
+        n_tiles = 2 * padded_width(n // 2) // 16 if gated else -(-n // 16)
+        if not (tiles.dtype == torch.uint8 and tuple(tiles.shape) == (n_tiles, k_tiles, 64, 16) and tiles.is_contiguous() and tiles.data_ptr() % 16 == 0
+                and scales.dtype == torch.uint8 and tuple(scales.shape) == (n_tiles, -(-k_tiles // 4), 64, 4) and scales.is_contiguous()
+                and scales.data_ptr() % 16 == 0):
+            raise ShapeError(f"the tiles of a [{n}, {k}] weight are uint8 [{n_tiles}, {k_tiles}, 64, 16], their scales [{n_tiles}, {-(-k_tiles // 4)}, 64, 4]")
+        return tuple.__new__(cls, (tiles, scales, int(n), int(k), bool(gated), n_tiles, k_tiles, device))
 
     @property
     def nbytes(self) -> int:
@@ -198,13 +271,13 @@ class MXWeight:
 
 def lay_weight(rows: MXRows, gated: bool = False) -> MXWeight:
     """The operand tiles of a weight given as "mxfp4" rows (quantize(w, "mxfp4")): a rearrangement at load time, the codes are untouched."""
-    _check_rows(rows, "weight")
-    _need(rows.form == "mxfp4", "weights are held in 4 bits (mxfp4)")
+    if type(rows) is not MXRows or rows.bits != 4:
+        raise ShapeError("weights are held in 4 bits: lay_weight takes mxfp4 rows")
     n, padded = rows.rows, rows.padded
-    _need(n > 0, "weight: no rows")
-    e, s = rows.elements, rows.scales
+    if n < 1 or (gated and n % 2):
+        raise ShapeError("a gated weight has as many gate rows as up rows" if n else "a weight without rows")
+    e, s = rows.elements, rows.scales.view(torch.uint8)
     if gated:
-        _need(n % 2 == 0, "a gated weight has as many gate rows as up rows")
         ff = n // 2
         more = padded_width(ff) - ff
         turns = lambda t: torch.nn.functional.pad(t.reshape(2, ff, -1), (0, 0, 0, more)).view(2, (ff + more) // 16, 16, -1).transpose(0, 1).flatten(0, 2)
@@ -216,63 +289,122 @@ def lay_weight(rows: MXRows, gated: bool = False) -> MXWeight:
     return MXWeight(tiles, scales, n, rows.width, gated)
 
 
-def _check_weight(w: MXWeight, x: MXRows, gated: bool) -> None:
-    _need(type(w) is MXWeight, f"the weight must be MXWeight (see lay_weight), got {type(w).__name__}")
-    _here(w.tiles, w.scales)
-    _need(w.gated == gated, "gate_up_act takes a weight laid out with gated=True, gemm one without")
-    _need(w.k == x.width, f"inner sizes differ ({x.width} vs {w.k})")
-    k_tiles = x.padded // TILE
-    n_tiles = 2 * padded_width(w.n // 2) // 16 if gated else -(-w.n // 16)
-    _need(w.tiles.dtype == torch.uint8 and tuple(w.tiles.shape) == (n_tiles, k_tiles, 64, 16) and w.tiles.is_contiguous()
-          and w.tiles.data_ptr() % 16 == 0 and w.scales.dtype == torch.uint8 and w.scales.is_contiguous()
-          and tuple(w.scales.shape) == (n_tiles, -(-k_tiles // 4), 64, 4) and w.scales.data_ptr() % 4 == 0,
-          f"the tiles of a [{w.n}, {w.k}] weight are [{n_tiles}, {k_tiles}, 64, 16], their scales [{n_tiles}, {-(-k_tiles // 4)}, 64, 4]")
+_EPI_F32, _EPI_GATE = F32, {"mxfp8": 2, "mxfp4": 3}                         # (sums leave as the type whose code this is)
+ROW_VARIANTS = (0, 1)                                                       # of up to 16 rows (mx_gemm_rows_kernel)
+# variant of mx_gemm_tiles_kernel -> rows, columns, workgroups a compute unit holds, us of 128 k for one workgroup alone and for a compute unit
+# that is as full as all others, for rows of 8 bits and of 4.  What the variants took (MI355X, 8 bits, us; the sizes are rows, N, K):
+#                           64x128  128x128  128x256  256x256  128x192
+#   512 x 2,560 x 9,728       33.7     40.2     48.0     78.7     43.6
+#   2,048 x 2,560 x 9,728     64.9     56.4     47.5     78.8     44.0
+#   2,048 x 6,144 x 2,560     34.8     29.9     33.5     31.4     33.5
+#   4,096 x 6,144 x 4,096    115.4     88.8     84.0     88.6     89.8
+#   4,096 x 4,096 x 12,288   209.9    163.2    148.2    137.5    168.2
+_TILES = {2: (32, 64, 2, 0.18, 0.40, 0.18, 0.40), 3: (64, 128, 1, 0.33, 0.33, 0.33, 0.33), 4: (128, 128, 2, 0.45, 0.85, 0.42, 0.81),
+          5: (128, 256, 1, 0.60, 0.77, 0.45, 0.70), 6: (256, 256, 1, 1.00, 1.40, 0.70, 1.00), 7: (128, 192, 1, 0.55, 0.62, 0.50, 0.62)}
+_UNITS = 256             # compute units
+_TILE_START_US = 2.5     # of a workgroup: its first loads and its results
+_SUM_US, _STACK_BYTES_A_US = 5.0, 5e6      # a launch more, which an eager caller pays the host for too; the stack written and read
 
 
-_EPI_F32, _EPI_BF16, _EPI_GATE = 0, 1, {"mxfp8": 2, "mxfp4": 3}
-_ROW_TILES = {0: 1, 1: 2, 2: 4}                                             # variant -> tiles of 16 rows (mx_gemm_rows_kernel)
-_TILE_SHAPES = {3: (64, 128), 4: (128, 128), 5: (128, 256), 6: (256, 256)}  # variant -> rows and columns (mx_gemm_tiles_kernel)
+def _tiles_us(variant: int, M: int, N: int, k_tiles: int, bits: int, splits: int) -> float:
+    """What a product is expected to take, as far as variants and parts of K are compared by it."""
+    rows, cols, held, *us = _TILES[variant]
+    alone, full = us[:2] if bits == 8 else us[2:]
+    groups = -(-M // rows) * -(-N // cols) * splits
+    share = groups / (_UNITS * held)
+    turns = max(1.0, share) if held > 1 else -(-groups // _UNITS)      # a unit that holds several starts the next one while others run
+    return turns * (4 * -(-k_tiles // (4 * splits)) * (alone + (full - alone) * min(1.0, share)) + _TILE_START_US)
 
 
-def _variant(M: int, n: int) -> int:
-    if M <= 64:
-        return 0 if M <= 16 else 1 if M <= 32 else 2
-    for v in (6, 5, 4):
-        rows, cols = _TILE_SHAPES[v]
-        if -(-M // rows) * -(-n // cols) >= 256:
-            return v
-    return 3
+@functools.lru_cache(maxsize=4096)
+def _plan(M: int, n_tiles: int, k_tiles: int, bits: int, gated: bool, whole: bool) -> tuple:
+    """(variant, parts of K, steps a part) for sizes; whole: the sums have to come whole."""
+    variant, splits = _choose(M, n_tiles, k_tiles, bits, gated, whole)
+    return variant, splits, _per_split(M, k_tiles, bits, variant, splits)
 
 
-def _launch(x: MXRows, w: MXWeight, epilogue: int, variant: int, splits: int, out, ldo: int, split_stride: int, out_scales, ldos: int, n: int,
-            vec: bool) -> None:
-    M = x.rows
-    k_tiles, bits = w.tiles.shape[1], BITS[x.form]
-    _need(variant not in _ROW_TILES or M <= 16 * _ROW_TILES[variant], f"variant {variant} takes {16 * _ROW_TILES.get(variant, 0)} rows")
-    steps = k_tiles if variant in _ROW_TILES or bits == 8 else k_tiles // 2     # what the kernel walks K in
+def _choose(M: int, n_tiles: int, k_tiles: int, bits: int, gated: bool, whole: bool) -> tuple:
+    N = 16 * n_tiles
+    if M <= 16 and not gated:
+        # us at 8 rows, pairs of columns tiles in 4 waves and K in as many parts as stand / the same whole / single tiles in 8 waves, whole:
+        # 2,560 x 4,096  4.1 (8) / 5.7 / 5.0;  2,560 x 9,728  5.7 (8) / 9.6 / 7.7;  6,144 x 2,560  4.6 (4) / 4.7 / 5.4;
+        # 10,240 x 5,120  8.6 (2) / 10.4 / 10.3
+        pairs = -(-n_tiles // 2)
+        if whole:
+            return (0 if pairs >= 192 else 1), 1
+        return 0, _even(min(max(1, round(640 / pairs)), 8, max(1, k_tiles // 4)), k_tiles)
+    found = []
+    for variant, (rows, _, *_) in _TILES.items():
+        if gated and variant in (2, 7):      # their waves own no whole block of 32 results
+            continue
+        for splits in (1,) if gated else (1, 2, 4, 8):
+            splits = _even(splits, k_tiles // 4)
+            us = _tiles_us(variant, M, N, k_tiles, bits, splits)
+            if splits > 1:
+                us += 8 * splits * M * N / _STACK_BYTES_A_US + (_SUM_US if whole else 0)
+            found.append((us, variant, splits))
+    _, variant, splits = min(found)
+    return variant, splits
+
+
+def _even(splits: int, steps: int) -> int:
+    """As many parts as `splits` parts of equal length make of `steps`, none of them empty."""
+    return -(-steps // -(-steps // min(splits, steps)))
+
+
+def _per_split(M: int, k_tiles: int, bits: int, variant: int, splits: int) -> int:
+    """Steps of K that a part walks; refuses what the kernel was not written for."""
+    few = variant in ROW_VARIANTS
+    if not few and variant not in _TILES:
+        raise ShapeError(f"no variant {variant}")
+    if few and M > 16:
+        raise ShapeError(f"variant {variant} takes 16 rows, got {M}")
+    steps = k_tiles if few else k_tiles // 4
+    if splits == 1:
+        return steps
     per_split = -(-steps // splits)
-    _need(splits >= 1 and (splits - 1) * per_split < steps, f"{splits} parts of {steps} steps: some would have none")
-    lib.call("arle_mx_gemm", bits, epilogue, variant, x.elements.data_ptr(), x.elements.stride(0), x.scales.data_ptr(), x.scales.stride(0),
-             w.tiles.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ldo, split_stride, _ptr(out_scales), ldos, M, n, w.tiles.shape[0], k_tiles,
-             splits, per_split, int(vec), _stream())
+    if splits < 1 or splits > 65535 or (splits - 1) * per_split >= steps:
+        raise ShapeError(f"{splits} parts of {steps} steps: some would have none")
+    return per_split
+
+
+def _checked(x: MXRows, w: MXWeight, gated: bool) -> int:
+    if type(x) is not MXRows or type(w) is not MXWeight:
+        raise ShapeError(f"products take MXRows and an MXWeight (see quantize, lay_weight), got {type(x).__name__} and {type(w).__name__}")
+    device = x[7]
+    if x[2] != w[3] or w[4] is not gated or w[7] != device:
+        if x.width != w.k:
+            raise ShapeError(f"inner sizes differ ({x.width} vs {w.k})")
+        if w.gated != gated:
+            raise ShapeError("gate_up_act takes a weight laid out with gated=True, gemm one without")
+        raise ShapeError(f"rows on cuda:{x.device}, the weight on cuda:{w.device}")
+    if device != _current():
+        _same_device(device)
+    return device
 
 
 def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partials_ok: bool = False, *, variant: int | None = None,
          splits: int | None = None) -> torch.Tensor:
     """x [T, K] . w [N, K]^T with sums of 32 bits -> [T, N] in `out_dtype`; with `partials_ok` possibly a float32 stack [S, T, N] whose
     sum over S, in order, is the product (as Linear's)."""
-    _check_rows(x)
-    _check_weight(w, x, False)
-    _need(out_dtype in (torch.float32, torch.bfloat16), "products come in float32 or bfloat16")
-    M, N, device = x.rows, w.n, x.elements.device
+    device = _checked(x, w, False)
+    code = _CODES.get(out_dtype)
+    if code is None:
+        raise ShapeError("products come in float32 or bfloat16")
+    elements, held, _, _, M, _, bits, _ = x
+    tiles, tile_scales, N, _, _, n_tiles, k_tiles, _ = w
+    on = _DEVICES.get(device) or _device(device)
     if M == 0:
-        return torch.empty((0, N), dtype=out_dtype, device=device)
+        return _empty(0, N, dtype=out_dtype, device=on)
     if variant is None:
-        variant = _variant(M, N)
-    splits = splits or 1
+        variant, splits, per_split = _plan(M, n_tiles, k_tiles, bits, False, not partials_ok)
+    else:
+        splits = splits or 1
+        per_split = _per_split(M, k_tiles, bits, variant, splits)
     parts = splits > 1
-    out = torch.empty((splits, M, N) if parts else (M, N), dtype=torch.float32 if parts else out_dtype, device=device)
-    _launch(x, w, _EPI_F32 if out.dtype == torch.float32 else _EPI_BF16, variant, splits, out, N, M * N, None, 0, N, N % 8 == 0)
+    out = _empty(splits, M, N, dtype=torch.float32, device=on) if parts else _empty(M, N, dtype=out_dtype, device=on)
+    _call("arle_mx_gemm", bits, _EPI_F32 if parts else code, variant, elements.data_ptr(), elements.stride(0), held.data_ptr(), held.stride(0),
+          tiles.data_ptr(), tile_scales.data_ptr(), out.data_ptr(), N, M * N, 0, 0, M, N, n_tiles, k_tiles, splits, per_split, N % 8 == 0, _stream(device))
     if parts and not partials_ok:
         return ops.sum_partials(out, out_dtype)
     return out
@@ -281,13 +413,21 @@ def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partia
 def gate_up_act(x: MXRows, w: MXWeight, form: str = "mxfp8", *, variant: int | None = None) -> MXRows:
     """silu(x . gate^T) * (x . up^T) in blocks, [T, ff] from a weight laid out with gated=True: the rows of the second half's product,
     made from the 32-bit sums in one kernel."""
-    _check_rows(x)
-    _check_weight(w, x, True)
-    _bits(form)
-    out = _empty_rows(x.rows, w.n // 2, form, x.elements.device)
-    if x.rows == 0:
+    device = _checked(x, w, True)
+    out_bits = BITS.get(form) or _bits(form)
+    elements, held, _, _, M, _, bits, _ = x
+    tiles, tile_scales, n, _, _, n_tiles, k_tiles, _ = w
+    out = _new_rows(M, n // 2, form, out_bits, device)
+    if M == 0:
         return out
     if variant is None:
-        variant = _variant(x.rows, 16 * w.tiles.shape[0])
-    _launch(x, w, _EPI_GATE[form], variant, 1, out.elements, out.elements.stride(0), 0, out.scales, out.scales.stride(0), 16 * w.tiles.shape[0], True)
+        variant, _, per_split = _plan(M, n_tiles, k_tiles, bits, True, True)
+    else:
+        if variant in (*ROW_VARIANTS, 2, 7):
+            raise ShapeError(f"variant {variant} makes no blocks")
+        per_split = _per_split(M, k_tiles, bits, variant, 1)
+    padded = out[5]
+    _call("arle_mx_gemm", bits, _EPI_GATE[form], variant, elements.data_ptr(), elements.stride(0), held.data_ptr(), held.stride(0), tiles.data_ptr(),
+          tile_scales.data_ptr(), out[0].data_ptr(), padded * out_bits // 8, 0, out[1].data_ptr(), padded // BLOCK, M, 16 * n_tiles, n_tiles, k_tiles, 1,
+          per_split, True, _stream(device))
     return out

@@ -51,7 +51,7 @@ def quantize(x: torch.Tensor, form: str):
 
 def unpack(rows) -> tuple:
     """(element codes a byte each, scale codes) of arle_amd's MXRows, on the CPU, padding included."""
-    e, s = rows.elements.cpu(), rows.scales.cpu()
+    e, s = rows.elements.view(torch.uint8).cpu(), rows.scales.view(torch.uint8).cpu()
     if rows.form == "mxfp4":
         e = torch.stack([e & 15, e >> 4], dim=-1).flatten(1)
     return e, s

@@ -3,18 +3,20 @@ import pytest
 import torch
 
 import plain_mx as plain
-from arle_amd.kernels import lib, mx, ops
+from arle_amd.kernels import mx, ops
 
 
 @pytest.fixture
 def no_gpu(monkeypatch):
     """CPU tensors pass, and no kernel may be asked for."""
-    monkeypatch.setattr(mx, "_here", lambda *t: None)
+    monkeypatch.setattr(mx, "_here", lambda *t: 0)
+    monkeypatch.setattr(mx, "_current", lambda: 0)
+    monkeypatch.setattr(mx, "_DEVICES", {d: torch.device("cpu") for d in (-1, 0)})
 
     def call(name, *args):
         raise AssertionError(f"{name} was launched")
 
-    monkeypatch.setattr(lib, "call", call)
+    monkeypatch.setattr(mx, "_call", call)
 
 
 def _rows(T, width, form="mxfp8", seed=0):
@@ -28,7 +30,7 @@ def _rows(T, width, form="mxfp8", seed=0):
 @pytest.mark.parametrize("T,width", [(0, 32), (1, 1), (3, 255), (5, 256), (2, 257), (4, 700)])
 def test_rows_from_codes(no_gpu, form, T, width):
     e, s, rows = _rows(T, width, form)
-    assert rows.rows == T and rows.padded % 256 == 0 and 0 <= rows.padded - width < 256
+    assert rows.rows == T and rows.padded % 512 == 0 and 0 <= rows.padded - width < 512
     got_e, got_s = plain.unpack(rows)
     assert torch.equal(got_e[:, :width], e) and not got_e[:, width:].any()
     blocks = s.shape[1]
@@ -59,7 +61,7 @@ def test_weight_tiles(no_gpu, n, k):
 def test_gated_weight_is_turns_of_sixteen(no_gpu, ff):
     e, s, rows = _rows(2 * ff, 64, "mxfp4")
     w = mx.lay_weight(rows, gated=True)
-    padded = -(-ff // 256) * 256
+    padded = -(-ff // 512) * 512
     assert w.n == 2 * ff and w.tiles.shape[0] == 2 * padded // 16
     codes, _ = plain.unpack(rows)
     for c in range(0, padded, 7):
@@ -77,6 +79,14 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def _e8(T, W):
+    return torch.zeros(T, W, dtype=torch.uint8).view(torch.float8_e4m3fn)
+
+
+def _s(T, B):
+    return torch.zeros(T, B, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+
+
 def test_refused_rows(no_gpu):
     bad = [
         lambda: mx.quantize(torch.zeros(2, 64), "mxfp6"),
@@ -91,9 +101,14 @@ def test_refused_rows(no_gpu):
         lambda: _rows(2, 64, "mxfp4")[2].elements_e4m3(),
         lambda: mx.values(torch.zeros(2, 64)),
         lambda: mx.values(_rows(2, 64)[2], torch.float16),
-        lambda: mx.values(mx.MXRows(torch.zeros(2, 300, dtype=torch.uint8)[:, 1:257], torch.zeros(2, 8, dtype=torch.uint8), 256, "mxfp8")),
-        lambda: mx.values(mx.MXRows(torch.zeros(2, 256, dtype=torch.uint8), torch.zeros(2, 8, dtype=torch.uint8), 300, "mxfp8")),
-        lambda: mx.values(mx.MXRows(torch.zeros(2, 256, dtype=torch.uint8), torch.zeros(1, 8, dtype=torch.uint8), 256, "mxfp8")),
+        lambda: mx.MXRows(_e8(2, 600)[:, 1:513], _s(2, 16), 512, "mxfp8"),
+        lambda: mx.MXRows(_e8(2, 513)[:, :512], _s(2, 16), 512, "mxfp8"),
+        lambda: mx.MXRows(_e8(2, 512), _s(2, 20)[:, :16], 512, "mxfp8"),
+        lambda: mx.MXRows(_e8(2, 512), _s(2, 16), 600, "mxfp8"),
+        lambda: mx.MXRows(_e8(2, 512), _s(1, 16), 512, "mxfp8"),
+        lambda: mx.MXRows(_e8(2, 512), _s(2, 16).view(torch.uint8), 512, "mxfp8"),
+        lambda: mx.MXRows(_e8(2, 512), _s(2, 16), 0, "mxfp8"),
+        lambda: mx.MXRows(_e8(2, 512), _s(2, 32), 1024, "mxfp4"),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(ops.ShapeError):
@@ -139,13 +154,31 @@ def test_refused_products(no_gpu):
         lambda: mx.gemm(x, mx.MXWeight(w.tiles[:1], w.scales, 40, 300)),
         lambda: mx.gemm(x, mx.MXWeight(w.tiles, w.scales, 60, 300)),
         lambda: mx.gemm(_rows(17, 300)[2], w, variant=0),                # more rows than the kernel holds
+        lambda: mx.gemm(x, w, variant=20),
+        lambda: mx.gate_up_act(x, wg, variant=7),
+        lambda: mx.gate_up_act(x, wg, variant=0),
         lambda: mx.gemm(x, w, variant=0, splits=5),                      # four steps of 128
-        lambda: mx.gemm(_rows(3, 300, "mxfp4")[2], w, variant=3, splits=3),   # two steps of 256
+        lambda: mx.gemm(_rows(3, 300, "mxfp4")[2], w, variant=3, splits=2),   # one round of 512
     ]
     for i, call in enumerate(bad):
         with pytest.raises(ops.ShapeError):
             call()
             pytest.fail(f"call {i} passed")
+
+
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_every_size_has_a_plan(bits, gated, whole):
+    """A variant that takes the rows, and parts of K of which none is empty."""
+    for M in (1, 2, 15, 16, 17, 31, 33, 64, 65, 100, 129, 500, 1000, 2048, 5000, 70000):
+        for n_tiles in (1, 3, 64, 96, 160, 384, 1216, 9496):
+            for k_tiles in (4, 8, 20, 32, 76, 96, 1000):
+                variant, splits, per_split = mx._plan(M, n_tiles, k_tiles, bits, gated, whole)
+                steps = k_tiles if variant in mx.ROW_VARIANTS else k_tiles // 4
+                assert splits >= 1 and (splits - 1) * per_split < steps <= splits * per_split
+                assert M <= 16 if variant in mx.ROW_VARIANTS else variant in mx._TILES
+                assert not gated or (splits == 1 and variant in (3, 4, 5, 6))
 
 
 def test_no_rows_launch_nothing(no_gpu):

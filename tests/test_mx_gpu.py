@@ -14,6 +14,10 @@ def _g(seed):
     return torch.Generator().manual_seed(seed)
 
 
+def _same(a, b):
+    return all(torch.equal(p, q) for p, q in zip(plain.unpack(a), plain.unpack(b)))
+
+
 def _wild(T, W, seed):
     """Rows whose blocks span the type's range: zeros, tiny and huge ones, ties, a maximum right at a border of two scales."""
     x = torch.randn(T, W, generator=_g(seed)) * torch.exp2(torch.randint(-100, 100, (T, W), generator=_g(seed + 1)).float() * (torch.rand(T, 1, generator=_g(seed + 2)) < 0.3))
@@ -55,7 +59,7 @@ def test_quantize_of_views(form):
     buf = torch.randn(9, 700, generator=_g(1)).bfloat16().to(DEV)
     for view in (buf[:, :256], buf[:, 8:264], buf[:, 3:260], buf[::2, 5:6], buf[1:4, 13:], buf[:, 4:260]):
         got, want = mx.quantize(view, form), mx.quantize(view.contiguous(), form)
-        assert torch.equal(got.elements, want.elements) and torch.equal(got.scales, want.scales)
+        assert _same(got, want)
 
 
 @pytest.mark.parametrize("form", FORMS)
@@ -68,7 +72,7 @@ def test_not_a_number_stays_in_its_block(form):
     bad[0, :32] = bad[1, 32:64] = bad[2, 96:] = True
     assert torch.equal(v.isnan(), bad)
     w = mx.lay_weight(mx.quantize(torch.randn(40, 128, generator=_g(3)).to(DEV), "mxfp4"))
-    for variant in range(7):
+    for variant in sorted(VARIANT_ROWS):
         y = mx.gemm(rows, w, torch.float32, variant=variant).cpu()
         assert y[:3].isnan().all() and y[3].isfinite().all()
 
@@ -124,7 +128,7 @@ def test_add_rmsnorm_of_picked_rows():
     got = mx.add_rmsnorm(res, delta, w, 1e-6, "mxfp8", rows=pick)
     assert torch.equal(res, before)
     whole = mx.add_rmsnorm(res, delta, w, 1e-6, "mxfp8")
-    assert torch.equal(got.elements, whole.elements[pick.long()]) and torch.equal(got.scales, whole.scales[pick.long()])
+    assert all(torch.equal(a, b[pick.long().cpu()]) for a, b in zip(plain.unpack(got), plain.unpack(whole)))
 
 
 # What a sum may be off by.  With an e4m3 operand the instruction aligns the products of 8 neighbouring k to the largest of them and drops what
@@ -148,7 +152,8 @@ def _operands(M, N, K, form, seed, spread=8):
     return (xe, xs), (we, ws), plain.dequantize(xe, xs, form), plain.dequantize(we, ws, "mxfp4")
 
 
-VARIANT_ROWS = {0: (1, 9, 16), 1: (1, 17, 32), 2: (3, 33, 64), 3: (1, 64, 65, 130), 4: (1, 127, 129, 300), 5: (5, 128, 200), 6: (2, 255, 257, 520)}
+VARIANT_ROWS = {0: (1, 9, 16), 1: (1, 8, 16), 2: (3, 33, 70), 3: (1, 64, 130), 4: (1, 127, 300), 5: (5, 128, 200), 6: (2, 255, 520), 7: (1, 128, 300)}
+GATED = (3, 4, 5, 6)
 
 
 @pytest.mark.parametrize("form", FORMS)
@@ -164,7 +169,7 @@ def test_gemm(form, variant, N, K):
         assert ((got - want).abs() <= off).all(), (M, N, K)
         got16 = mx.gemm(rows, weight, torch.bfloat16, variant=variant).cpu().double()
         assert ((got16 - want).abs() <= off + 2.0**-8 * (want.abs() + off)).all(), (M, N, K)
-        steps = rows.padded // (128 if variant < 3 or form == "mxfp8" else 256)
+        steps = rows.padded // (128 if variant in mx.ROW_VARIANTS else 512)
         for splits in (2, 3):
             if (splits - 1) * -(-steps // splits) < steps:
                 parts = mx.gemm(rows, weight, torch.float32, partials_ok=True, variant=variant, splits=splits)
@@ -192,7 +197,7 @@ def test_gemm_of_whole_numbers_is_exact(form, variant, N, K):
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("out", FORMS)
 @pytest.mark.parametrize("ff,K", [(1, 40), (32, 256), (100, 300), (256, 130), (300, 1100)])
-@pytest.mark.parametrize("variant", sorted(VARIANT_ROWS))
+@pytest.mark.parametrize("variant", GATED)
 def test_gate_up_act(form, out, variant, ff, K):
     for M in VARIANT_ROWS[variant][1:]:
         x, w, xv, wv = _operands(M, 2 * ff, K, form, M + ff, spread=4)
@@ -223,10 +228,10 @@ def test_strided_rows_and_slices():
     x = mx.quantize(torch.randn(40, 512, generator=_g(1)).to(DEV))
     w = mx.lay_weight(mx.quantize(torch.randn(70, 512, generator=_g(2)).to(DEV), "mxfp4"))
     whole = mx.gemm(x, w, torch.float32, variant=2)
-    assert torch.equal(mx.gemm(x[7:29], w, torch.float32, variant=2), whole[7:29])
+    assert torch.equal(mx.gemm(x.part(7, 29), w, torch.float32, variant=2), whole[7:29])
     wide_e, wide_s = torch.zeros(40, 1024, dtype=torch.uint8, device=DEV), torch.zeros(40, 64, dtype=torch.uint8, device=DEV)
-    wide_e[:, 256:768], wide_s[:, 4:20] = x.elements, x.scales
-    apart = mx.MXRows(wide_e[:, 256:768], wide_s[:, 4:20], 512, "mxfp8")
+    wide_e[:, 256:768], wide_s[:, 16:32] = x.elements.view(torch.uint8), x.scales.view(torch.uint8)
+    apart = mx.MXRows(wide_e[:, 256:768].view(torch.float8_e4m3fn), wide_s[:, 16:32].view(torch.float8_e8m0fnu), 512, "mxfp8")
     assert torch.equal(mx.gemm(apart, w, torch.float32, variant=2), whole)
     assert torch.equal(mx.values(apart), mx.values(x))
 
@@ -234,6 +239,20 @@ def test_strided_rows_and_slices():
 def test_every_kernel_of_few_or_many_rows_gives_the_same_row_whatever_stands_beside_it():
     x = mx.quantize(torch.randn(300, 700, generator=_g(1)).to(DEV))
     w = mx.lay_weight(mx.quantize(torch.randn(90, 700, generator=_g(2)).to(DEV), "mxfp4"))
-    for variant, rows in ((0, 16), (1, 32), (2, 64), (3, 300), (4, 300), (5, 300), (6, 300)):
-        whole = mx.gemm(x[:rows], w, torch.float32, variant=variant)
-        assert torch.equal(mx.gemm(x[rows - 1:rows], w, torch.float32, variant=variant)[0], whole[-1])
+    for variant, rows in ((0, 16), (1, 16), (2, 64), (3, 300), (4, 300), (5, 300), (6, 300), (7, 300)):
+        whole = mx.gemm(x.part(0, rows), w, torch.float32, variant=variant)
+        assert torch.equal(mx.gemm(x.part(rows - 1, rows), w, torch.float32, variant=variant)[0], whole[-1])
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 2560, 4096), (8, 48, 9728), (16, 6144, 2560), (17, 2560, 2560), (40, 6144, 2610), (100, 1531, 2610), (600, 2560, 4096)])
+@pytest.mark.parametrize("form", FORMS)
+def test_chosen_variants(form, M, N, K):
+    """Whatever the sizes choose: whole sums, a stack where it may be one, and the two alike."""
+    x, w, xv, wv = _operands(M, N, K, form, M)
+    rows, weight = mx.rows_from_codes(*(t.to(DEV) for t in x), K, form), mx.lay_weight(mx.rows_from_codes(*(t.to(DEV) for t in w), K, "mxfp4"))
+    want, off = xv @ wv.T, _sum_error(form, K) * (xv.abs() @ wv.abs().T)
+    got = mx.gemm(rows, weight).cpu().double()
+    assert ((got - want).abs() <= off + 2.0**-8 * (want.abs() + off)).all()
+    stack = mx.gemm(rows, weight, torch.float32, partials_ok=True)
+    total = stack.cpu().double().sum(0) if stack.dim() == 3 else stack.cpu().double()
+    assert ((total - want).abs() <= off).all()
