@@ -75,6 +75,10 @@ def build_parser() -> argparse.ArgumentParser:
                          "table to FILE (read again with ARLE_AMD_PRODUCT_TABLE=FILE); about a minute")
     ap.add_argument("--no-weight-tiles", action="store_true",
                     help="do not keep the second, decode-friendly copy of the projection weights")
+    ap.add_argument("--weight-form", choices=["mxfp4"], default=None,
+                    help="hold the projections of attention and feed-forward in 4 bits with a power of two for every 32 weights")
+    ap.add_argument("--row-form", choices=["mxfp8", "mxfp4"], default="mxfp8",
+                    help="the rows that meet such weights: e4m3 in blocks of 32, or 4 bits too")
     sub = ap.add_subparsers(dest="command")
     run = sub.add_parser("run", help="run a single prompt and exit")
     src = run.add_mutually_exclusive_group()
@@ -122,7 +126,7 @@ def _run(argv=None) -> int:
               page_size=args.page_size, seed=args.seed, cuda_graph=not args.no_cuda_graph,
               mem_fraction_static=args.mem_fraction_static,
               weight_tiles=False if args.no_weight_tiles else None, warm_up=args.warm_up,
-              tune_products=args.tune_products or False)
+              tune_products=args.tune_products or False, weight_form=args.weight_form, row_form=args.row_form)
     if args.prompt_ids:
         prompt = [int(t) for t in args.prompt_ids.replace(" ", "").split(",") if t]
     else:

@@ -86,7 +86,8 @@ class LLM:
                  chunked_prefill_size: int | None = None, max_num_batched_tokens: int = 16384,
                  max_prefill_tokens: int | None = None, prefill_max_requests: int | None = None, seed: int = 42,
                  cuda_graph: bool = True, weight_tiles: bool | None = None, mem_fraction_static: float = 0.85,
-                 async_overlap: bool = True, warm_up: bool = False, tune_products: bool | str = False):
+                 async_overlap: bool = True, warm_up: bool = False, tune_products: bool | str = False,
+                 weight_form: str | None = None, row_form: str = "mxfp8"):
         """model: a model folder, or an Engine that is already built.
 
         kv_cache_tokens: tokens the paged cache holds over all live requests.  Default: sized from the GPU's
@@ -101,6 +102,7 @@ class LLM:
         num_slots: requests that run at a time; None: as many requests of max_seq_len tokens as the cache holds, from 4
         to 128 (the reference's --num-slots left unset).
         cuda_graph, weight_tiles: as for Engine (captured steps; the decode-friendly second copy of the weights).
+        weight_form, row_form: as for Engine (projections held in 4 bits, the rows that meet them in 8 or 4).
         async_overlap: decode steps are launched from the last step's tokens on the GPU, and those are read back
         while the new step runs (SchedulerConfig.async_overlap); the tokens are the same either way.
         tune_products: measure which kernel runs each of this model's matrix products fastest at each row count and
@@ -124,7 +126,8 @@ class LLM:
                                              page_size=page_size or DEFAULT_PAGE_SIZE,
                                              max_tokens=kv_cache_tokens, max_slots=num_slots,
                                              max_request_tokens=max_seq_len, cuda_graph=cuda_graph,
-                                             weight_tiles=weight_tiles, mem_fraction_static=mem_fraction_static)
+                                             weight_tiles=weight_tiles, mem_fraction_static=mem_fraction_static,
+                                             weight_form=weight_form, row_form=row_form)
         self.model_dir = model if isinstance(model, str) else None
         self.seed = seed
         cfg = SchedulerConfig.runtime_defaults(self.engine.cache.max_slots)

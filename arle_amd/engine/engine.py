@@ -19,10 +19,10 @@ from ..cache.manager import (CacheManager, OutOfPages, PagedNeed, all_leaves, ca
                              slots_for_tokens, state_bytes_per_slot)
 from ..config.registry import detect_architecture, load_model_config
 from ..models.decoder import DEBUG_DUMP_ENV, build_model, expected_checkpoint_tensors
-from ..parts.base import Runtime
+from ..parts.base import Runtime, lookup
 from ..weights.loader import load_weights
 from ..weights.random_init import random_weights
-from ..kernels import ops
+from ..kernels import mx, ops
 from .batch import DeviceToken, StepEntry, build_step_batch, packed_size
 
 DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32,
@@ -67,7 +67,8 @@ class Engine:
                  num_pages: int | None = None, max_slots: int | None = 4,
                  max_request_tokens: int | None = None, cuda_graph: bool = True,
                  weight_tiles: bool | None = None, mem_fraction_static: float = DEFAULT_MEM_FRACTION_STATIC,
-                 product_table=None):
+                 product_table=None, weight_form: str | None = None, row_form: str = "mxfp8",
+                 _owns_tensors: bool = False):
         """
         max_tokens: tokens the cache holds over all live requests (num_pages = ceil(max_tokens / page_size)
             unless num_pages is given).  With neither, the pool is sized from the GPU's memory as the
@@ -84,6 +85,11 @@ class Engine:
         product_table: a table (or the path of its file) that says which kernel runs each matrix product at each
             row count, measured for this model's widths (`bench.py --tune-products`); without one, the rules that
             were measured at the Qwen3-4B, 8B and 32B widths decide.  The table is the process's, not this engine's.
+        weight_form: "mxfp4" holds the projections of attention and feed-forward in 4 bits, blocks of 32 numbers along
+            the input with a power of two each (4.25 bits a weight), made from the checkpoint's weights when the engine is built;
+            norms, embedding, head, cache and attention stay as they are.  The rows that meet them are made into blocks by the kernel in front
+            (norm, activation) as `row_form` says: "mxfp8" (e4m3) or "mxfp4".  For designs whose mixers and feed-forwards have
+            that form (the Qwen3 dense decoder), in bfloat16.  None: as the checkpoint holds them.
         weight_tiles: hold every bfloat16 projection weight a second time in the layout that the few-rows
             kernels stream fastest (decode steps about a tenth faster, twice the weight memory), and the projections
             that a norm and another projection stand behind (o and down, the last down not) a third time where they have 769 to
@@ -96,12 +102,18 @@ class Engine:
         self.spec = spec
         if product_table is not None:
             ops.load_product_table(product_table)
+        if weight_form is not None:
+            self._check_weight_form(spec, weight_form, row_form)
         if weight_tiles is None:
             held = sum(t.numel() * t.element_size() for t in tensors.values() if t.dim() == 2)
             weight_tiles = 2 * held * 3 <= torch.cuda.get_device_properties(self.device).total_memory
         self.rt = Runtime(device=self.device, act_dtype=self.dtype,
-                          weight_tiles=bool(weight_tiles) and self.dtype == torch.bfloat16)
+                          weight_tiles=bool(weight_tiles) and self.dtype == torch.bfloat16,
+                          weight_form=weight_form, row_form=row_form)
         self.model = build_model(spec, tensors, self.rt)
+        if weight_form is not None and _owns_tensors:      # what has a form of its own now is no longer needed; the cache is sized by what is free
+            tensors.clear()
+            torch.cuda.empty_cache()
         needs, readers = self.model.cache_needs()
         self.kv_bytes_per_token = cache_bytes_per_token(needs, self.dtype)
         if max_slots is None:
@@ -146,6 +158,18 @@ class Engine:
         self.graph_replays = 0
         self._warm_total = None       # the contexts' total that a step of `warm_up` stands for
 
+    def _check_weight_form(self, spec, weight_form: str, row_form: str) -> None:
+        if weight_form != "mxfp4":
+            raise EngineError(f"unknown weight_form {weight_form!r}; use mxfp4, or None for the checkpoint's own")
+        if row_form not in mx.BITS:
+            raise EngineError(f"unknown row_form {row_form!r}; use {' or '.join(mx.BITS)}")
+        if self.dtype != torch.bfloat16:
+            raise EngineError(f"weight_form {weight_form!r} needs dtype bfloat16")
+        for layer in spec.layers:
+            for role, part in (("mixer", layer.mixer), ("feed_forward", layer.feed_forward), *layer.parts.values()):
+                if part is not None and weight_form not in lookup(role, part.kind).weight_forms:
+                    raise EngineError(f"weight_form {weight_form!r} is not built for the {role.replace('_', '-')} {part.kind!r}")
+
     # -- construction -----------------------------------------------------------------
     @classmethod
     def from_folder(cls, model_dir: str, *, dtype="bfloat16", device=None, **cache_args) -> "Engine":
@@ -154,7 +178,7 @@ class Engine:
         spec = arch.recipe(config, stops)
         dev = _device(device)
         tensors = load_weights(model_dir, expected_checkpoint_tensors(spec), dev, parse_dtype(dtype))
-        engine = cls(spec, tensors, dtype=dtype, device=dev, **cache_args)
+        engine = cls(spec, tensors, dtype=dtype, device=dev, _owns_tensors=True, **cache_args)
         engine.config, engine.architecture = config, arch.name
         return engine
 
@@ -166,7 +190,7 @@ class Engine:
         spec = arch.recipe(config, ())
         dev = _device(device)
         tensors = random_weights(spec, seed, std, norm_std, parse_dtype(dtype), device=dev)
-        engine = cls(spec, tensors, dtype=dtype, device=dev, **cache_args)
+        engine = cls(spec, tensors, dtype=dtype, device=dev, _owns_tensors=True, **cache_args)
         engine.config, engine.architecture = config, arch.name
         return engine
 

@@ -19,9 +19,9 @@ import math
 import torch
 
 from ..cache.manager import PagedNeed
-from ..kernels import ops
+from ..kernels import mx, ops
 from .base import Part, WeightDecl, register
-from .linear import Linear
+from .linear import Linear, MXLinear
 
 
 @register("mixer", "paged_attention")
@@ -30,6 +30,7 @@ class PagedAttention(Part):
     position (PartSpec), window (int | None), scale (float | None: 1/sqrt(head_dim))."""
 
     graph_safe = True  # positions, slots and lengths are read on the GPU; launches depend on shapes only
+    weight_forms = ("mxfp4",)
 
     @classmethod
     def declare_weights(cls, params):
@@ -72,12 +73,14 @@ class PagedAttention(Part):
         if not (wq.dtype == wk.dtype == wv.dtype):
             raise ValueError("q, k and v projections must be stored in one type")
         self.q_width, self.kv_width = self.nq * self.D, self.nkv * self.D
-        self.qkv = Linear(torch.cat([wq, wk, wv], dim=0).contiguous(), rt.weight_tiles)
+        fused = torch.cat([wq, wk, wv], dim=0).contiguous()
+        self.reads_form = rt.row_form if rt.weight_form else None      # of the rows that the norm in front leaves
+        self.qkv = MXLinear(fused, rt.row_form) if rt.weight_form else Linear(fused, rt.weight_tiles)
         # for a layer that reads another layer's cache: the q rows of the fused matrix, no copy (head_dim is a
         # multiple of 16, so the q rows are whole operand tiles too)
-        self.q_only = Linear(self.qkv.weight[: self.q_width], packed=self.qkv.tiles)
+        self.q_only = self.qkv.first(self.q_width) if rt.weight_form else Linear(self.qkv.weight[: self.q_width], packed=self.qkv.tiles)
         self.leaves_late = False
-        self.o = Linear(tensors["o"], rt.weight_tiles)
+        self.o = MXLinear(tensors["o"], rt.row_form) if rt.weight_form else Linear(tensors["o"], rt.weight_tiles)
         # steps of single decoded tokens run norm, rotation and cache write inside the attention's kernel where it
         # has that form (ops.attn_decode_prep_supported); params["fold_preparation"] = False keeps the two kernels
         self.folds_preparation = bool(params.get("fold_preparation", True))
@@ -91,7 +94,7 @@ class PagedAttention(Part):
         return self.declare_cache(self.params)
 
     def products(self):
-        if self.qkv.weight.dtype != torch.bfloat16:
+        if self.rt.weight_form or self.qkv.weight.dtype != torch.bfloat16:
             return []
         return [("qkv", self.qkv.out_features, self.qkv.in_features, False, "norm"),
                 ("o", self.o.out_features, self.o.in_features, False, "norm")]
@@ -112,11 +115,11 @@ class PagedAttention(Part):
 
     @property
     def reads_scaled(self) -> bool:
-        return self.qkv.weight.dtype == torch.bfloat16
+        return not self.rt.weight_form and self.qkv.weight.dtype == torch.bfloat16
 
     def leave_late(self) -> None:
         """A norm that can run the output projection stands behind it, and a reader of ops.ScaledRows behind that."""
-        if self.rt.weight_tiles:
+        if self.rt.weight_tiles and not self.rt.weight_form:
             self.o.lay_strips()
             self.leaves_late = self.o.strips is not None
 
@@ -132,8 +135,10 @@ class PagedAttention(Part):
         return [(self.qkv.out_features, self.qkv.in_features, False)]
 
     def forward(self, x, batch, cache, late: bool = False):
-        """x [T, H] (or ops.ScaledRows, see takes_scaled) -> [T, H], or a float32 stack [S, T, H] to be added in order (see Linear);
-        late: possibly the output projection for the norm behind it to run."""
+        """x [T, H] (or ops.ScaledRows, see takes_scaled, or mx.MXRows, see reads_form) -> [T, H], or a float32 stack [S, T, H] to be added
+        in order (see Linear); late: possibly the output projection for the norm behind it to run."""
+        in_blocks = type(x) is mx.MXRows
+        rows, dtype, device = (x.rows, self.rt.act_dtype, x.elements.device) if in_blocks else (x.shape[0], x.dtype, x.device)
         Q, KV = self.q_width, self.kv_width
         self.position.ensure_positions(batch.max_position + 1)
         cos, sin, rot = self.position.fused_rotary()
@@ -149,9 +154,9 @@ class PagedAttention(Part):
         projected = (self.qkv if cache.writes else self.q_only)(x, partials_ok=fused)
         if (fused and cache.writes and batch.max_qlen == 1 and self.folds_preparation
                 and (projected.dim() == 3 or projected.dtype == torch.bfloat16)
-                and ops.attn_decode_prep_supported(x.dtype, self.D, cache.page_size, self.nq // self.nkv, rot)):
+                and ops.attn_decode_prep_supported(dtype, self.D, cache.page_size, self.nq // self.nkv, rot)):
             # single decoded tokens: the attention's kernel sums, norms, rotates and writes to the cache itself
-            out = torch.empty((x.shape[0], Q), dtype=x.dtype, device=x.device)
+            out = torch.empty((rows, Q), dtype=dtype, device=device)
             ops.attn_decode_prep(projected, out, cache.k_pages, cache.v_pages, cache.block_table, batch.seg_row0,
                                  batch.seg_slot, batch.seg_start, max_kv_len=batch.max_position + 1,
                                  num_q_heads=self.nq, num_kv_heads=self.nkv, head_dim=self.D, page_size=cache.page_size,
@@ -160,7 +165,7 @@ class PagedAttention(Part):
                                  total_kv_len=getattr(batch, "total_context", 0) or None, carry=getattr(batch, "carry", None))
             return self.o.late(out) if late and self.leaves_late else self.o(out, partials_ok=True)
         if projected.dim() == 3:
-            q = torch.empty((x.shape[0], Q), dtype=x.dtype, device=x.device)
+            q = torch.empty((rows, Q), dtype=dtype, device=device)
             ops.qk_prep(q, None, None, q_weight=self.q_norm, k_weight=self.k_norm, cos=cos, sin=sin,
                         rotary_dim=rot, parts=projected, **to_cache, **common)
         else:
@@ -179,7 +184,7 @@ class PagedAttention(Part):
                 self.position.apply(q, k, batch.positions, self.nq, nkv)
                 if to_cache:
                     ops.qk_prep(q, k, v, **to_cache, **common)
-        out = torch.empty((x.shape[0], Q), dtype=q.dtype, device=q.device)
+        out = torch.empty((rows, Q), dtype=q.dtype, device=q.device)
         paged_attention(q, out, cache, batch, num_q_heads=self.nq, num_kv_heads=self.nkv,
                         head_dim=self.D, scale=self.scale, window=self.window or 0)
         return self.o.late(out) if late and self.leaves_late else self.o(out, partials_ok=True)

@@ -12,6 +12,7 @@ Interfaces (T = tokens of the packed step, H = hidden size, A = activation dtype
                 A delta is A[T,H], or a float32 stack [S,T,H] of partial sums to be added in the order
                 of S (what a matrix product with K split over workgroups leaves behind).
 * position      `fused_rotary() -> (cos, sin, rotary_dim) | None`;  `apply(q, k, positions)` in place.
+                With `form` (where `takes_form`) the rows come in blocks, `mx.MXRows`, for a reader whose `reads_form` names it.
 * mixer         `cache_need() -> PagedNeed | StateNeed | {name: need, ...} | None` (and, so that a model's cache can
                 be sized from its description alone, the class method `declare_cache(params)` with the same answer;
                 `reader_cache_need()` / `declare_reader_cache(params)`: what it keeps in an entry that reads another
@@ -71,6 +72,10 @@ class Runtime:
     # keep a second copy of every bfloat16 projection weight as operand tiles, the layout that the few-rows
     # kernels stream fastest (twice the weight memory; the library keeps reading the rows)
     weight_tiles: bool = False
+    # "mxfp4": projections hold their weights in 4 bits with a power of two for every 32 of them (kernels/mx.py) and meet rows in blocks
+    # too, of the form `row_form` ("mxfp8" or "mxfp4"); None: as the checkpoint holds them
+    weight_form: str | None = None
+    row_form: str = "mxfp8"
 
     @property
     def is_f32(self) -> bool:
@@ -94,6 +99,8 @@ class Part:
     # shape, reading whatever varies (positions, slots, lengths) from GPU memory: only then may the
     # engine replay the part from a captured graph.
     graph_safe = False
+    # The forms beside the checkpoint's own that this part can hold its projections in (Runtime.weight_form).
+    weight_forms = ()
 
     @classmethod
     def declare_weights(cls, params: dict) -> dict:

@@ -28,9 +28,16 @@ class PreNormBlock:
         self.norm_mixer = norms["mixer_in"]
         self.norm_ffn = norms["ffn_in"] if feed_forward is not None else None
         self._late = [{}, {}]
+        # what a norm is asked for beside its sums: rows in blocks where the part behind reads them
+        self._form = [self._asked_form(self.norm_mixer, mixer), self._asked_form(self.norm_ffn, feed_forward)]
         self.late_pairs = []      # (a part whose last projection is left to a norm, the part behind that norm)
         if self.norm_ffn is not None:
             self._leave_late(0, mixer, self.norm_ffn, feed_forward)
+
+    @staticmethod
+    def _asked_form(norm, reader) -> dict:
+        form = getattr(reader, "reads_form", None)
+        return {"form": form} if form is not None and getattr(norm, "takes_form", False) else {}
 
     def followed_by(self, block) -> None:
         """`block` may come next in the schedule: its first norm is what the last projection here can be left to."""
@@ -46,25 +53,25 @@ class PreNormBlock:
                 self.late_pairs.append((part, reader))
 
     @staticmethod
-    def _add_norm(norm, residual, delta, reader, cache_view=None):
+    def _add_norm(norm, residual, delta, reader, form, cache_view=None):
         if isinstance(delta, LateProduct):
             takes = getattr(reader, "takes_scaled", None)
             if takes is not None and hasattr(norm, "add_late") and takes(residual.shape[0], cache_view):
                 return norm.add_late(residual, delta)
             delta = delta.now()
-        return norm.add_norm(residual, delta)
+        return norm.add_norm(residual, delta, **form)
 
     def forward(self, residual, delta, batch, cache_view):
         if residual.shape[0] > STRIP_ROWS:      # nothing is left to a norm here, and a step's first pass is bound by the host
-            m = self.mixer.forward(self.norm_mixer.add_norm(residual, delta), batch, cache_view)
+            m = self.mixer.forward(self.norm_mixer.add_norm(residual, delta, **self._form[0]), batch, cache_view)
             if self.norm_ffn is None:
                 return residual, m
-            return residual, self.feed_forward.forward(self.norm_ffn.add_norm(residual, m))
-        a = self._add_norm(self.norm_mixer, residual, delta, self.mixer, cache_view)
+            return residual, self.feed_forward.forward(self.norm_ffn.add_norm(residual, m, **self._form[1]))
+        a = self._add_norm(self.norm_mixer, residual, delta, self.mixer, self._form[0], cache_view)
         m = self.mixer.forward(a, batch, cache_view, **self._late[0])
         if self.norm_ffn is None:
             return residual, m
-        b = self._add_norm(self.norm_ffn, residual, m, self.feed_forward)
+        b = self._add_norm(self.norm_ffn, residual, m, self.feed_forward, self._form[1])
         return residual, self.feed_forward.forward(b, **self._late[1])
 
 

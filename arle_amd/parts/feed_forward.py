@@ -12,7 +12,7 @@ import torch
 
 from ..kernels import ops
 from .base import Part, WeightDecl, register
-from .linear import Linear
+from .linear import Linear, MXLinear
 
 
 @register("feed_forward", "swiglu")
@@ -22,6 +22,7 @@ class SwiGLU(Part):
     what the gate passes through before it multiplies up)."""
 
     graph_safe = True  # launches depend on shapes only, never on the values of a step
+    weight_forms = ("mxfp4",)
 
     @classmethod
     def declare_weights(cls, params):
@@ -39,6 +40,15 @@ class SwiGLU(Part):
         gate, up = tensors["gate"], tensors["up"]
         if gate.dtype != up.dtype:
             raise ValueError("gate and up projections must be stored in one type")
+        self.leaves_late = False
+        self.reads_form = rt.row_form if rt.weight_form else None      # of the rows that the norm in front leaves
+        if rt.weight_form:
+            if self.act != 0:
+                raise ValueError(f"projections in {rt.weight_form} are built for the silu gate, not for {name!r}")
+            self.block = 0
+            self.gate_up = MXLinear(torch.cat([gate, up], dim=0), rt.row_form, gated=True)
+            self.down = MXLinear(tensors["down"], rt.row_form)
+            return
         # bfloat16: rows interleaved in blocks of 16 (16 gate rows, the 16 matching up rows, ...), so
         # that one tile of the decode kernel holds both halves of 16 outputs and applies the activation
         # itself.  Otherwise gate rows first, then up rows.
@@ -49,7 +59,6 @@ class SwiGLU(Part):
         else:
             fused = torch.cat([gate, up], dim=0)
         self.gate_up = Linear(fused.contiguous(), rt.weight_tiles)
-        self.leaves_late = False
         self.down = Linear(tensors["down"], rt.weight_tiles)
 
     @property
@@ -58,7 +67,7 @@ class SwiGLU(Part):
 
     def leave_late(self) -> None:
         """A norm that can run the down projection stands behind it, and a reader of ops.ScaledRows behind that."""
-        if self.rt.weight_tiles and not self.float32_out:
+        if self.rt.weight_tiles and not self.float32_out and not self.rt.weight_form:
             self.down.lay_strips()
             self.leaves_late = self.down.strips is not None
 
@@ -75,15 +84,17 @@ class SwiGLU(Part):
                                                       tiled=self.gate_up.tiles is not None, fused=True)
 
     def products(self):
-        if self.gate_up.weight.dtype != torch.bfloat16:
+        if self.rt.weight_form or self.gate_up.weight.dtype != torch.bfloat16:
             return []
         return [("gate_up", self.gate_up.out_features, self.gate_up.in_features, bool(self.block), None),
                 ("down", self.down.out_features, self.down.in_features, False, "norm")]
 
     def forward(self, x, late: bool = False):
-        """x [T, H] (or ops.ScaledRows, see takes_scaled) -> [T, H], or a float32 stack [S, T, H] to be added in order (see Linear);
-        late: possibly the down projection for the norm behind it to run."""
-        if type(x) is ops.ScaledRows:
+        """x [T, H] (or ops.ScaledRows, see takes_scaled, or mx.MXRows, see reads_form) -> [T, H], or a float32 stack [S, T, H] to be added in
+        order (see Linear); late: possibly the down projection for the norm behind it to run."""
+        if self.rt.weight_form:
+            act = self.gate_up.gate_up(x)
+        elif type(x) is ops.ScaledRows:
             act = ops.gate_up_act(x.rows, self.gate_up.weight, self.gate_up.tiles, scaled=x)
         elif self.block:
             act = ops.gate_up_act(x, self.gate_up.weight, self.gate_up.tiles, self.act)   # one product with the activation, or two kernels

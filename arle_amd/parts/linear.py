@@ -22,12 +22,15 @@ which is worth a fifth of their time on MI355X.  The library needs the rows, so 
 A projection whose result goes into the residual can be left to the norm behind it (`late`): for up to eight rows product, add
 and norm are then one kernel (ops.gemm_strips), for which `lay_strips` holds the weight in that kernel's layout too where the
 tiles are not that layout already.
+
+`MXLinear` holds its weight in 4 bits in blocks of 32 and meets rows in blocks too: those that a norm or an activation in front has left so, or
+its own from rows in bfloat16.
 """
 from __future__ import annotations
 
 import torch
 
-from ..kernels import ops
+from ..kernels import mx, ops
 
 
 class LateProduct:
@@ -91,3 +94,39 @@ class Linear:
         if x.dtype != torch.bfloat16:
             raise ops.ShapeError(f"a bfloat16 weight needs bfloat16 activations, got {x.dtype}")
         return ops.gemm_bf16(x, w, out_dtype, partials_ok=partials_ok, tiles=self.tiles)
+
+
+class MXLinear:
+    """A projection whose weight is held as "mxfp4" (kernels/mx.py), a quarter of bfloat16 and a bit; the weight it is made from is not kept.
+
+    gated: the weight is the gate's rows and then the up's, for `gate_up`."""
+
+    weight = tiles = strips = None      # of a projection in bfloat16
+
+    def __init__(self, weight: torch.Tensor, row_form: str, gated: bool = False):
+        if weight.dim() != 2:
+            raise ValueError("a projection weight must be an [out, in] matrix")
+        self.out_features, self.in_features = weight.shape
+        self.row_form = row_form
+        self.held = mx.lay_weight(mx.quantize(weight, "mxfp4"), gated=gated)
+
+    def first(self, rows: int) -> "MXLinear":
+        """The projection to the first `rows` outputs (a multiple of 16), no copy."""
+        if rows % 16 or self.held.gated:
+            raise ValueError("part of a weight is whole operand tiles of a plain one")
+        part = object.__new__(MXLinear)
+        part.out_features, part.in_features, part.row_form = rows, self.in_features, self.row_form
+        part.held = mx.MXWeight(self.held.tiles[:rows // 16], self.held.scales[:rows // 16], rows, self.in_features)
+        return part
+
+    def rows(self, x) -> mx.MXRows:
+        return x if type(x) is mx.MXRows else mx.quantize(x, self.row_form)
+
+    def __call__(self, x, out_dtype: torch.dtype | None = None, partials_ok: bool = False) -> torch.Tensor:
+        """x [T, in] in bfloat16 or float32, or mx.MXRows -> [T, out] in `out_dtype` (default: bfloat16); with `partials_ok` possibly a
+        float32 stack, as Linear's."""
+        return mx.gemm(self.rows(x), self.held, out_dtype or torch.bfloat16, partials_ok)
+
+    def gate_up(self, x) -> mx.MXRows:
+        """silu(gate x) * (up x) in blocks, the rows of the projection behind."""
+        return mx.gate_up_act(self.rows(x), self.held, self.row_form)

@@ -6,7 +6,7 @@ The weight keeps the type the checkpoint stores it in (bfloat16 or float32).
 """
 from __future__ import annotations
 
-from ..kernels import ops
+from ..kernels import mx, ops
 from .base import Part, WeightDecl, register
 
 
@@ -47,8 +47,15 @@ class RMSNorm(Part):
                            act_dtype=self.rt.act_dtype if rounded else None, mult=self.add_scale)
         return out if rounded else residual
 
-    def add_norm(self, residual, delta, rows=None):
-        """residual (float32) += delta, then the norm of it; delta None: just the norm."""
+    @property
+    def takes_form(self) -> bool:
+        """Whether `add_norm` can leave its rows in blocks."""
+        return self.width <= mx.MAX_WIDTH
+
+    def add_norm(self, residual, delta, rows=None, form=None):
+        """residual (float32) += delta, then the norm of it; delta None: just the norm.  form: the rows in blocks (mx.MXRows)."""
+        if form is not None:
+            return mx.add_rmsnorm(residual, delta, self.weight, self.eps, form, rows=rows)
         if delta is None:
             return ops.rmsnorm(residual, self.weight, self.eps, self.rt.act_dtype, rows=rows)
         return ops.add_rmsnorm(residual, delta, self.weight, self.eps, self.rt.act_dtype, rows=rows)

@@ -1296,6 +1296,8 @@ def main() -> int:
                          "next step is launched from the tokens on the GPU, as the scheduler does)")
     ap.add_argument("--no-weight-tiles", action="store_true",
                     help="without the second copy of the projection weights that the few-rows kernels stream")
+    ap.add_argument("--weight-form", choices=["mxfp4"], default=None, help="projections of the default workload held in 4 bits")
+    ap.add_argument("--row-form", choices=["mxfp8", "mxfp4"], default="mxfp8", help="the rows that meet them")
     ap.add_argument("--no-parts", action="store_true",
                     help="skip the breakdown of the step's time by part of the model (a profiled step)")
     ap.add_argument("--parts-only", action="store_true",
@@ -1379,7 +1381,8 @@ def main() -> int:
     t0 = time.time()
     engine = Engine.from_config("Qwen3ForCausalLM", config, seed=0, std=0.02, dtype=args.dtype,
                                 page_size=PAGE, max_tokens=(max_batch + 1) * longest, max_slots=max_batch + 1,
-                                max_request_tokens=longest, weight_tiles=False if args.no_weight_tiles else None)
+                                max_request_tokens=longest, weight_tiles=False if args.no_weight_tiles else None,
+                                weight_form=args.weight_form, row_form=args.row_form)
     print(f"[bench] engine ready in {time.time() - t0:.1f} s", file=sys.stderr, flush=True)
     gen = torch.Generator().manual_seed(1234)
     sampler = Sampler(engine.device)       # the product's sampler: greedy rows are one argmax kernel, read back on its own stream
@@ -1523,12 +1526,16 @@ def main() -> int:
                      "frac": round(achieved / PEAK_HBM_GBS, 4)},
         "points": points,
     }
-    if not args.no_parts and dkey == "bf16":
+    if not args.no_parts and dkey == "bf16" and not args.weight_form:
         line.update(parts_in_a_child_process(args))
         # the parts come from a second, profiled run: their sums stand beside the timed steps they are read against
         if isinstance(line.get("prefill_parts_us"), dict):
             line["prefill_parts_us"]["timed_step"] = round(prefill["ms"] * 1e3, 1)
             line["decode_parts_us"]["timed_step"] = round(ms_per_step * 1e3, 1)
+    if args.weight_form:
+        line["metric"] += f", projections in {args.weight_form}, rows in {args.row_form}"
+        line["config"].update(weight_form=args.weight_form, row_form=args.row_form)
+        line.pop("roofline")      # of the bytes of bfloat16 weights
     if args.batch != 8:
         line["metric"] = line["metric"].replace("batch 8", f"batch {args.batch}")
     print(json.dumps(line))

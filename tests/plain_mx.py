@@ -70,3 +70,35 @@ def gated(x, w):
     y = x @ w.T
     gate, up = y.chunk(2, dim=1)
     return gate * torch.sigmoid(gate) * up
+
+
+def round_rows(x, form):
+    """The numbers that rows in blocks stand for."""
+    return dequantize(*quantize(x, form), form)
+
+
+def qwen3_logits(weights, cfg, tokens, weight_form, row_form):
+    """Logits of the plain Qwen3 decoder in 64 bits whose projections hold their weights as `weight_form` and meet rows as `row_form` (None: as
+    they are): the norms' rows, the attention's output and the activation's products."""
+    import plain_qwen3 as q
+
+    w = {n: t.double() for n, t in weights.items()}
+    held = {n: round_rows(t, weight_form) if weight_form and ("_proj.weight" in n) else t for n, t in w.items()}
+    rows = (lambda x: round_rows(x, row_form)) if row_form else (lambda x: x)
+    T, eps = len(tokens), cfg["rms_norm_eps"]
+    nq, nkv, D = cfg["num_attention_heads"], cfg["num_key_value_heads"], cfg["head_dim"]
+    cos, sin = q.rope_cos_sin(range(T), D, cfg["rope_theta"], dtype=torch.float64)
+    h = q.embedding(w["model.embed_tokens.weight"], tokens)
+    for i in range(cfg["num_hidden_layers"]):
+        p = f"model.layers.{i}."
+        x = rows(q.rms_norm(h, w[p + "input_layernorm.weight"], eps))
+        of = lambda name, heads: (x @ held[f"{p}self_attn.{name}_proj.weight"].T).view(T, heads, D)
+        qs = q.prepare_heads(of("q", nq), w[p + "self_attn.q_norm.weight"], eps, cos, sin)
+        ks = q.prepare_heads(of("k", nkv), w[p + "self_attn.k_norm.weight"], eps, cos, sin)
+        a = q.causal_attention(qs, ks, of("v", nkv), nkv).reshape(T, nq * D)
+        h = h + rows(a) @ held[p + "self_attn.o_proj.weight"].T
+        x = rows(q.rms_norm(h, w[p + "post_attention_layernorm.weight"], eps))
+        act = q.silu(x @ held[p + "mlp.gate_proj.weight"].T) * (x @ held[p + "mlp.up_proj.weight"].T)
+        h = h + rows(act) @ held[p + "mlp.down_proj.weight"].T
+    f = q.rms_norm(h, w["model.norm.weight"], eps)
+    return f @ (w["model.embed_tokens.weight"] if cfg["tie_word_embeddings"] else w["lm_head.weight"]).T

@@ -187,3 +187,29 @@ def test_no_rows_launch_nothing(no_gpu):
     assert mx.gemm(none, w).shape == (0, 40) and mx.gate_up_act(none, wg).rows == 0
     assert mx.quantize(torch.zeros(0, 64)).rows == 0 and mx.values(none).shape == (0, 300)
     assert mx.add_rmsnorm(torch.zeros(0, 64), None, torch.ones(64), 1e-6).rows == 0
+
+
+def test_designs_without_that_form_are_refused():
+    from arle_amd import models  # noqa: F401
+    from arle_amd.config.registry import detect_architecture
+    from arle_amd.engine.engine import Engine, EngineError
+
+    import tiny
+    import tiny_gufasun
+
+    qwen3 = detect_architecture({"architectures": [tiny.ARCH]})
+    spec = qwen3.recipe(qwen3.config_class.from_dict(tiny.TINY["A"][0]), ())
+    engine = object.__new__(Engine)
+    engine.dtype = torch.bfloat16
+    engine._check_weight_form(spec, "mxfp4", "mxfp8")
+    for form, rows in (("int4", "mxfp8"), ("mxfp4", "bf16")):
+        with pytest.raises(EngineError):
+            engine._check_weight_form(spec, form, rows)
+    engine.dtype = torch.float32
+    with pytest.raises(EngineError, match="bfloat16"):
+        engine._check_weight_form(spec, "mxfp4", "mxfp8")
+    engine.dtype = torch.bfloat16
+    raw = next(v for v in vars(tiny_gufasun).values() if isinstance(v, dict) and "layers" in v)
+    other = detect_architecture(raw)
+    with pytest.raises(EngineError, match="not built for"):
+        engine._check_weight_form(other.recipe(other.config_class.from_dict(raw), ()), "mxfp4", "mxfp8")
