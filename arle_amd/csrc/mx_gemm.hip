@@ -2,9 +2,11 @@
 // blocks of 32 along K with a power of two each (mx.h).  v_mfma_scale takes elements and scales as they are: an operand is 32
 // elements a lane and one scale byte a lane, the sum of a block's products times the two scales, added in 32 bits.
 //
-// W is laid out once as operand tiles of 16 columns x 128 k, [ceil(N/16)][K/128][64][16 bytes], lane 16 g + i: W[16 t + i][128 s + 32 g
-// .. + 31], one contiguous kilobyte a wave and load; its scales as [ceil(N/16)][ceil(K/512)][64] words, byte s % 4 of lane 16 g + i
-// for that lane's block of tile s.  K is padded with zeros to a multiple of 512 on both sides.
+// W is laid out once as operand tiles of 16 columns x 128 k, [K/128][ceil(N/16)][64][16 bytes], lane 16 g + i of tile (s, t): W[16 t + i][128 s + 32
+// g .. + 31], one contiguous kilobyte a wave and load; its scales as [K/512][ceil(N/16)][64] words, byte s % 4 of lane 16 g + i
+// for that lane's block of tile s.  (K outermost: what a step fetches of neighbouring columns lies together and meets all channels of a
+// cache.  With N outermost a step's tiles lie multiples of 4 KB apart: 2,048 x 2,560 x 9,728 with X in e2m1 39.5 instead of 35.1 us, gate|up of 64 x 9,728 x
+// 2,560 13.3 instead of 12.1, with X in e4m3 46.6 / 46.2 and 512 x 2,560 x 9,728 26.2 / 25.1; up to 16 rows the same.)  K is padded with zeros to a multiple of 512 on both sides.
 //
 // With W as the first operand (rows of the result are W's columns) a lane ends up with four neighbouring columns of one row.
 // Operand layouts of the second operand's lane (row i, group g): e2m1 32 neighbouring k from 32 g on, as the first; e4m3 16 neighbouring
@@ -23,20 +25,19 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMxF32 = 0, kMxBf16 = 1, kMxGate8 = 2, kMxGate4 = 3;   // what leaves: sums, or silu(gate) * up in blocks
 
+// (96 bytes: a launch with more than about 100 takes the host 0.7 us more)
 struct MxArgs {
   const uint8_t* x;
-  int64_t ldx;            // bytes between rows of elements
   const uint8_t* xs;
-  int64_t ldxs;
   const uint8_t* w;
   const uint32_t* ws;
   void* out;
-  int64_t ldo, split_stride;
   uint8_t* out_scales;
-  int64_t ldos;
+  int ldx, ldxs;          // bytes between rows of elements, of scales
+  int ldo, ldos;          // between rows of results (elements) and of their scales; parts of K lie M x ldo apart
   int M, N, n_tiles, k_tiles;
+  int pitch;              // tiles between a step of W and the next
   int per_split;          // steps of K that one workgroup walks
-  int vec;                // rows of `out` take whole 16-byte stores
   int m_blocks, n_blocks;
 };
 
@@ -57,8 +58,8 @@ template <int EPI>
 __device__ __forceinline__ void mx_store_sums(const MxArgs& a, int split, int row, int n, mx_f32x4 v) {
   if (row >= a.M || n >= a.N) return;
   if constexpr (EPI == kMxF32) {
-    float* o = static_cast<float*>(a.out) + split * a.split_stride + static_cast<int64_t>(row) * a.ldo + n;
-    if (a.vec && n + 4 <= a.N) {
+    float* o = static_cast<float*>(a.out) + static_cast<int64_t>(split) * a.M * a.ldo + static_cast<int64_t>(row) * a.ldo + n;
+    if ((a.ldo & 7) == 0 && n + 4 <= a.N) {
       *reinterpret_cast<mx_f32x4*>(o) = v;
       return;
     }
@@ -67,7 +68,7 @@ __device__ __forceinline__ void mx_store_sums(const MxArgs& a, int split, int ro
       if (n + e < a.N) o[e] = v[e];
   } else {
     bf16* o = static_cast<bf16*>(a.out) + static_cast<int64_t>(row) * a.ldo + n;
-    if (a.vec && n + 4 <= a.N) {
+    if ((a.ldo & 7) == 0 && n + 4 <= a.N) {
       *reinterpret_cast<uint2*>(o) = uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
       return;
     }
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(WAVES* kWave) void mx_gemm_rows_kernel(const MxArgs
   __shared__ mx_f32x4 parts[WAVES][CT][kTile];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4;
-  const int ct0 = blockIdx.x * CT, k_tiles = a.k_tiles, k_groups = k_tiles / 4;
+  const int ct0 = blockIdx.x * CT, k_tiles = a.k_tiles;
   const int begin = blockIdx.y * a.per_split, end = min(begin + a.per_split, k_tiles);
   const int n = (end - begin - wave + WAVES - 1) / WAVES;      // this wave's tiles: begin + wave, + WAVES, ...; none or less: none
 
@@ -100,8 +101,8 @@ __global__ __launch_bounds__(WAVES* kWave) void mx_gemm_rows_kernel(const MxArgs
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     const int64_t tile = min(ct0 + c, a.n_tiles - 1);
-    wp[c] = a.w + tile * k_tiles * 1024 + lane * 16;
-    wsp[c] = a.ws + tile * k_groups * 64 + lane;
+    wp[c] = a.w + tile * 1024 + lane * 16;
+    wsp[c] = a.ws + tile * 64 + lane;
   }
   const int64_t row = min(i, a.M - 1);                          // lanes past the rows: the last row again, their sums are dropped
   const uint8_t* xp = a.x + row * a.ldx + 16 * g;
@@ -113,8 +114,8 @@ __global__ __launch_bounds__(WAVES* kWave) void mx_gemm_rows_kernel(const MxArgs
   auto load = [&](int t, Step& s) {
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      s.w[c] = *reinterpret_cast<const u32x4*>(wp[c] + static_cast<int64_t>(t) * 1024);
-      s.ws[c] = wsp[c][(t >> 2) * 64];
+      s.w[c] = *reinterpret_cast<const u32x4*>(wp[c] + static_cast<int64_t>(t) * a.pitch * 1024);
+      s.ws[c] = wsp[c][static_cast<int64_t>(t >> 2) * a.pitch * 64];
     }
 #pragma unroll
     for (int half = 0; half < kParts; ++half) s.x[half] = *reinterpret_cast<const u32x4*>(xp + static_cast<int64_t>(t) * (16 * BITS) + 64 * half);
@@ -169,10 +170,15 @@ __global__ __launch_bounds__(WAVES* kWave) void mx_gemm_rows_kernel(const MxArgs
 //   * X: rows of 128 or 64 bytes, 16-byte pieces exchanged by the row: piece c of row r at c ^ (r / 2 % 8), or c ^ (r / 4 % 4), so that neighbouring
 //     lanes fetch a row's contiguous bytes and sixteen lanes that read a column of pieces meet all 64 banks.
 //   * W: its tiles as they are, a kilobyte a load; a 32-column operand is two tiles' runs of 256 bytes.
-//   * A step is 2 MT groups of TN products.  In every group the operands of the next group are read and a few of the batch's loads are sent, in
+//   * A step is 2 MT groups of TN products.  In every group the operands of a group behind are read and a few of the batch's loads are sent, in
 //     an order that is pinned (left to itself the compiler gathers two steps' reads in front of two steps' products).  The step's
-//     barrier stands before its last group, whose operands are in registers: behind it the next step's stage is there and this
+//     barrier stands before its last groups, whose operands are in registers: behind it the next step's stage is there and this
 //     step's is free, and the next step's first operands are read while the last products run.
+//
+// What bounds it (MI355X): 4,096 x 4,096 x 12,288 in 256 x 256, one workgroup a compute unit, takes 135 us, 3.0 PFLOP/s; the same without its
+// loads 115, with nothing but its loads 81 (14.5 TB/s from the L2s), the matrix cores are busy 87 % of the time and the clock is down to
+// 1.9 GHz.  Smaller tiles are bound by their loads: 2,048 x 2,560 x 9,728 in 128 x 192 44 us, without loads 34, loads alone 32; 4,096 x 6,144 x
+// 4,096 with X in e2m1, twice the products a second, 64, 50 and 50.  Waves that only load (one or two a workgroup) cannot send fast enough: 45 -> 55 us.
 template <int BITS, int MT, int TN, int RW, int CW, int STAGES, int WAVES_A_SIMD, int EPI>
 __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_kernel(const MxArgs a) {
   constexpr bool kGate = EPI == kMxGate8 || EPI == kMxGate4;
@@ -182,7 +188,9 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
   constexpr int kXBytes = kRows * kRowBytes, kStage = kXBytes + kTiles * 1024;
   constexpr int kXScales = (kRows < 64 ? 64 : kRows) * 16, kScales = kXScales + kTiles * 256;   // of a round
   constexpr int XD = kXBytes / 1024 / kWaves, WD = kTiles / kWaves, kBatch = XD + WD;   // loads of a wave and step
-  constexpr int kGroups = 2 * MT;
+  // operands are read kAhead groups before their products (us, one / two: 256 x 256 at gate|up of 4,096 x 12,288 x 4,096 307 / 302, 128 x 192 at
+  // 2,048 x 2,560 x 9,728 45.4 / 46.2)
+  constexpr int kGroups = 2 * MT, kAhead = MT >= 4 ? 2 : 1, kRing = kAhead == 1 ? 2 : 4;
   static_assert(XD * kWaves * 1024 == kXBytes && WD * kWaves == kTiles && kTiles % 4 == 0, "whole loads a wave");
   static_assert(STAGES >= 2 && STAGES <= 8, "a step's batch is sent STAGES - 1 steps ahead; a ninth would overtake a round's scales");
   extern __shared__ __align__(16) unsigned char lds[];
@@ -212,7 +220,7 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
   }
   const uint8_t* w0[WD];
 #pragma unroll
-  for (int q = 0; q < WD; ++q) w0[q] = a.w + static_cast<int64_t>(min(tile0 + WD * wave + q, a.n_tiles - 1)) * k_tiles * 1024;
+  for (int q = 0; q < WD; ++q) w0[q] = a.w + static_cast<int64_t>(min(tile0 + WD * wave + q, a.n_tiles - 1)) * 1024;
   // a round's scales are kilobytes too: 64 rows of X or four tiles of W; which is which is a matter of addresses, as a branch in the loop
   // would part it into pieces between which the compiler moves products; a load too many is the last one again
   constexpr int kXItems = kXScales / 1024, kItems = kXItems + kTiles / 4, SD = (kItems + kWaves - 1) / kWaves;
@@ -225,8 +233,8 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
     const bool of_x = item < kXItems;
     s0[q] = of_x ? a.xs + static_cast<int64_t>(m0) * a.ldxs : reinterpret_cast<const uint8_t*>(a.ws);
     s_off[q] = of_x ? static_cast<uint32_t>(min(64 * item + lane, a.M - 1 - m0)) * static_cast<uint32_t>(a.ldxs)
-                    : static_cast<uint32_t>(min(tile0 + 4 * (item - kXItems) + (lane >> 4), a.n_tiles - 1) * rounds) * 256u + (lane & 15) * 16;
-    s_step[q] = of_x ? 16 : 256;
+                    : static_cast<uint32_t>(min(tile0 + 4 * (item - kXItems) + (lane >> 4), a.n_tiles - 1)) * 256u + (lane & 15) * 16;
+    s_step[q] = of_x ? 16 : a.pitch * 256;
     s_to[q] = item * 1024;
   }
   // step s of this part; past its end the last step again, so that every step has as many loads
@@ -240,7 +248,7 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
     if (i < XD)
       load_to_lds_16(x0 + abs * kRowBytes, x_off[i], to + (XD * wave + i) * 1024);
     else
-      load_to_lds_16(w0[i - XD] + abs * 1024, lane * 16, to + kXBytes + (WD * wave + i - XD) * 1024);
+      load_to_lds_16(w0[i - XD] + abs * (static_cast<int64_t>(a.pitch) * 1024), lane * 16, to + kXBytes + (WD * wave + i - XD) * 1024);
   };
 
   mx_f32x16 acc[MT][TN];
@@ -267,20 +275,28 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
     return *reinterpret_cast<const u32x4*>(from + (x_at ^ (BITS == kMx8 ? 64 * kk + 32 * part : 32 * kk)) + 32 * kRowBytes * t);
   };
   auto read_w = [&](const unsigned char* from, int kk, int tn) { return *reinterpret_cast<const u32x4*>(from + w_at + 2048 * tn + 512 * kk); };
-  u32x4 xs[MT];          // of a round: a row's sixteen bytes, turned so that this lane's blocks are bytes 0 and 2 of the step's word
-  uint32_t ws[TN][2];
-  auto read_scales = [&](int round) {
+  struct Scales {
+    u32x4 x[MT];           // of a round: a row's sixteen bytes; in use turned so that this lane's blocks are bytes 0 and 2 of the step's word
+    uint32_t w[TN][2];
+  };
+  auto read_scales = [&](int round, Scales& to) {
     const unsigned char* sc = lds_scales + (round & 1) * kScales;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xs[t] = *reinterpret_cast<const u32x4*>(sc + (wr * 32 * MT + 32 * t + j) * 16) >> (8u * h);
+    for (int t = 0; t < MT; ++t) to.x[t] = *reinterpret_cast<const u32x4*>(sc + (wr * 32 * MT + 32 * t + j) * 16);
 #pragma unroll
     for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
       for (int half = 0; half < 2; ++half)
-        ws[tn][half] = *reinterpret_cast<const uint32_t*>(sc + kXScales + (wc * 2 * TN + 2 * tn + (j >> 4)) * 256 + (16 * (2 * half + h) + (j & 15)) * 4);
+        to.w[tn][half] = *reinterpret_cast<const uint32_t*>(sc + kXScales + (wc * 2 * TN + 2 * tn + (j >> 4)) * 256 + (16 * (2 * half + h) + (j & 15)) * 4);
   };
-  XOperand xo[2];
+  XOperand xo[kRing];
   u32x4 wo[2][TN];
+  Scales scales, scales_next;
+  auto use_scales = [&](const Scales& from) {
+    scales = from;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) scales.x[t] >>= 8u * h;
+  };
   constexpr int kFormat = BITS == kMx8 ? 0 : 4;
   auto batch_landed = [] { asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * kBatch) : "memory"); };   // all but the youngest batches
 
@@ -292,9 +308,12 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
   }
   batch_landed();
   __syncthreads();
-  read_scales(0);
+  read_scales(0, scales_next);
+  use_scales(scales_next);
 #pragma unroll
-  for (int part = 0; part < (BITS == kMx8 ? 2 : 1); ++part) xo[0].part[part] = read_x(lds, 0, 0, part);
+  for (int g = 0; g < kAhead; ++g)
+#pragma unroll
+    for (int part = 0; part < (BITS == kMx8 ? 2 : 1); ++part) xo[g].part[part] = read_x(lds, g / MT, g % MT, part);
 #pragma unroll
   for (int tn = 0; tn < TN; ++tn) wo[0][tn] = read_w(lds, 0, tn);
   unsigned char *now = lds, *last = lds + (STAGES - 1) * kStage;     // the stage of this step; where the batch goes
@@ -307,23 +326,24 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         const int kk = g / MT, t = g % MT;
-        if (g == kGroups - 1) {
+        if (g == kGroups - kAhead) {
           batch_landed();
           __syncthreads();
+          if constexpr (u == 3) read_scales(r + 1, scales_next);
         }
-        const unsigned char* from = g == kGroups - 1 ? next : now;
-        const int gn = (g + 1) % kGroups;
-        const int xscale = static_cast<int>(xs[t][u]);
-        const mx_i32x8 x = xo[g & 1].whole();
+        const unsigned char* from = g >= kGroups - kAhead ? next : now;
+        const int gn = (g + kAhead) % kGroups;
+        const int xscale = static_cast<int>(scales.x[t][u]);
+        const mx_i32x8 x = xo[g % kRing].whole();
 #pragma unroll
         for (int tn = 0; tn < TN; ++tn) {
           // in front of every product a piece of the operands of the group behind, and a load of the batch here and there
           constexpr int kParts = BITS == kMx8 ? 2 : 1;
 #pragma unroll
           for (int part = 0; part < kParts; ++part)
-            if (TN == 1 || tn == part) xo[(g + 1) & 1].part[part] = read_x(from, gn / MT, gn % MT, part);
-          if (t == MT - 1) wo[(kk + 1) & 1][tn] = read_w(from, (kk + 1) & 1, tn);
-          constexpr int kSlots = (kGroups - 1) * TN;
+            if (TN == 1 || tn == part) xo[(g + kAhead) % kRing].part[part] = read_x(from, gn / MT, gn % MT, part);
+          if (gn % MT == 0) wo[gn / MT][tn] = read_w(from, gn / MT, tn);
+          constexpr int kSlots = (kGroups - kAhead) * TN;
           const int slot_at = g * TN + tn;
           if (slot_at < kSlots) {
 #pragma unroll
@@ -332,15 +352,15 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
           }
           // the byte of W's scale word is the step inside the round, that of X's the half
           if (kk == 0)
-            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[0][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(ws[tn][0]), 0,
+            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[0][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(scales.w[tn][0]), 0,
                                                                          xscale);
           else
-            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[1][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(ws[tn][1]), 2,
+            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[1][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(scales.w[tn][1]), 2,
                                                                          xscale);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if constexpr (u == 3) read_scales(r + 1);
+      if constexpr (u == 3) use_scales(scales_next);
       last = now;
       now = next;
     };
@@ -398,12 +418,12 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
         for (int p = 0; p < 2; ++p)
 #pragma unroll
           for (int q = 0; q < 2; ++q) mx_store4<kBits>(mine + j * kPitch, 32 * b + 16 * p + 8 * q + 4 * h, mx_pack4<kBits>(v[p][q], code));
-        if (h == 0 && row0 + j < a.M) a.out_scales[(row0 + j) * a.ldos + n0 / 64 + b] = static_cast<uint8_t>(code);
+        if (h == 0 && row0 + j < a.M) a.out_scales[static_cast<int64_t>(row0 + j) * a.ldos + n0 / 64 + b] = static_cast<uint8_t>(code);
       }
-      leave(row0, static_cast<uint8_t*>(a.out) + row0 * a.ldo + n0 / 2 * kBits / 8, a.ldo);
+      leave(row0, static_cast<uint8_t*>(a.out) + static_cast<int64_t>(row0) * a.ldo + n0 / 2 * kBits / 8, a.ldo);
     }
   } else {
-    const bool whole = a.vec && n0 + 32 * TN <= a.N;      // the same in all lanes
+    const bool whole = (a.ldo & 7) == 0 && n0 + 32 * TN <= a.N;      // the same in all lanes
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       const int row0 = m0 + 32 * (MT * wr + t);
@@ -421,7 +441,7 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
           for (int q = 0; q < 4; ++q)
             *reinterpret_cast<uint2*>(mine + j * kPitch + (32 * tn + 8 * q + 4 * h) * 2) =
                 uint2{pack_bf16x2(acc[t][tn][4 * q], acc[t][tn][4 * q + 1]), pack_bf16x2(acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3])};
-        leave(row0, reinterpret_cast<unsigned char*>(static_cast<bf16*>(a.out) + row0 * a.ldo + n0), a.ldo * 2);
+        leave(row0, reinterpret_cast<unsigned char*>(static_cast<bf16*>(a.out) + static_cast<int64_t>(row0) * a.ldo + n0), static_cast<int64_t>(a.ldo) * 2);
       } else {
 #pragma unroll
         for (int tn = 0; tn < TN; ++tn) {
@@ -429,7 +449,7 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
           for (int q = 0; q < 4; ++q)
             *reinterpret_cast<mx_f32x4*>(mine + j * kPitch + (8 * q + 4 * h) * 4) =
                 mx_f32x4{acc[t][tn][4 * q], acc[t][tn][4 * q + 1], acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3]};
-          leave(row0, reinterpret_cast<unsigned char*>(static_cast<float*>(a.out) + blockIdx.y * a.split_stride + row0 * a.ldo + n0 + 32 * tn), a.ldo * 4);
+          leave(row0, reinterpret_cast<unsigned char*>(static_cast<float*>(a.out) + (static_cast<int64_t>(blockIdx.y) * a.M + row0) * a.ldo + n0 + 32 * tn), static_cast<int64_t>(a.ldo) * 4);
         }
       }
     }
@@ -480,11 +500,12 @@ int mx_launch(int variant, const MxArgs& a, int splits, hipStream_t s) {
 using namespace arle;
 
 extern "C" int arle_mx_gemm(int bits, int epilogue, int variant, const void* x, long long ldx, const void* xs, long long ldxs, const void* w,
-                            const void* ws, void* out, long long ldo, long long split_stride, void* out_scales, long long ldos, int M, int N,
-                            int n_tiles, int k_tiles, int splits, int per_split, int vec, void* stream) {
-  const MxArgs a = {static_cast<const uint8_t*>(x), ldx, static_cast<const uint8_t*>(xs), ldxs, static_cast<const uint8_t*>(w),
-                    static_cast<const uint32_t*>(ws), out, ldo, split_stride, static_cast<uint8_t*>(out_scales), ldos, M, N, n_tiles, k_tiles,
-                    per_split, vec, 0, 0};
+                            const void* ws, void* out, long long ldo, void* out_scales, long long ldos, int M, int N, int n_tiles, int k_tiles,
+                            int pitch, int splits, int per_split, void* stream) {
+  const MxArgs a = {static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w), static_cast<const uint32_t*>(ws),
+                    out, static_cast<uint8_t*>(out_scales), static_cast<int>(ldx), static_cast<int>(ldxs), static_cast<int>(ldo),
+                    static_cast<int>(ldos), M, N, n_tiles, k_tiles, pitch, per_split, 0, 0};
+  static_assert(sizeof(MxArgs) <= 96, "see MxArgs");
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto with = [&](auto b) {
     constexpr int kBits = decltype(b)::value;

@@ -1,6 +1,9 @@
 // Rows to microscaled rows and back: quantisation, the numbers that elements stand for, and the residual's addition with
 // the root-mean-square norm whose rows go straight into blocks.
 //
+// `threads` is the block's width as an argument: a kernel that asks the runtime for it takes 256 bytes of hidden arguments along, and a launch
+// with more than about 100 bytes takes the host 0.7 us more (3.5 instead of 2.8).
+//
 // A microscaled row is padded with zeros to a multiple of 512 numbers (`padded`), so that the products behind it walk whole
 // steps; every byte of it is written here.
 #include "mx.h"
@@ -12,8 +15,8 @@ namespace arle {
 // ---- quantisation: a thread owns eight columns of kRows rows, four lanes a block
 template <typename T, int BITS, bool ALIGNED, int kRows>
 __global__ __launch_bounds__(512) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ elements,
-                                                           uint8_t* __restrict__ scales, int rows, int width, int padded) {
-  const int unit = blockIdx.y * blockDim.x + threadIdx.x;   // of eight columns
+                                                           uint8_t* __restrict__ scales, int rows, int width, int padded, int threads) {
+  const int unit = blockIdx.y * threads + threadIdx.x;   // of eight columns
   const int col = 8 * unit;
   if (col >= padded) return;                                 // whole blocks: padded is a multiple of 32
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
@@ -54,8 +57,8 @@ __global__ __launch_bounds__(512) void mx_quantize_kernel(const T* __restrict__ 
 // ---- the numbers that the elements stand for: a thread owns eight columns of one row
 template <typename TOut, int BITS>
 __global__ __launch_bounds__(512) void mx_values_kernel(const uint8_t* __restrict__ elements, int64_t ld, const uint8_t* __restrict__ scales,
-                                                         int64_t ld_scales, TOut* __restrict__ out, int width) {
-  const int col = 8 * (blockIdx.y * blockDim.x + threadIdx.x);
+                                                         int64_t ld_scales, TOut* __restrict__ out, int width, int threads) {
+  const int col = 8 * (blockIdx.y * threads + threadIdx.x);
   if (col >= width) return;
   const int64_t row = blockIdx.x;
   const float s = mx_scale(scales[row * ld_scales + col / kMxBlock]);
@@ -126,15 +129,16 @@ __global__ __launch_bounds__(THREADS) void mx_norm_kernel(float* __restrict__ re
     float4 sum[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) sum[j] = mx_ld4<TD, ALIGNED>(d, 4 * (threadIdx.x + j * THREADS), width);
-    for (int p = 1; p < n_delta; p += 3) {    // three parts in flight; past the last one the last again, not added
-      float4 e[3][VPT];
+    constexpr int kAhead = VPT == 1 ? 7 : 3;      // parts on their way; past the last one nothing is fetched
+    for (int p = 1; p < n_delta; p += kAhead) {
+      float4 e[kAhead][VPT];
 #pragma unroll
-      for (int u = 0; u < 3; ++u)
+      for (int u = 0; u < kAhead; ++u)
+        if (p + u < n_delta)
 #pragma unroll
-        for (int j = 0; j < VPT; ++j)
-          e[u][j] = mx_ld4<TD, ALIGNED>(d + min(p + u, n_delta - 1) * delta_stride, 4 * (threadIdx.x + j * THREADS), width);
+          for (int j = 0; j < VPT; ++j) e[u][j] = mx_ld4<TD, ALIGNED>(d + (p + u) * delta_stride, 4 * (threadIdx.x + j * THREADS), width);
 #pragma unroll
-      for (int u = 0; u < 3; ++u)
+      for (int u = 0; u < kAhead; ++u)
         if (p + u < n_delta)
 #pragma unroll
           for (int j = 0; j < VPT; ++j) {
@@ -188,12 +192,22 @@ int mx_norm_launch(float* residual, const void* delta, int n_delta, int64_t delt
 #define ARLE_MX_NORM(THREADS, VPT)                                                                                       \
   mx_norm_kernel<TD, TW, BITS, ALIGNED, THREADS, VPT><<<n_rows, THREADS, 0, s>>>(                                        \
       residual, static_cast<const TD*>(delta), n_delta, delta_stride, static_cast<const TW*>(w), elements, scales, rows, width, padded, eps)
+  // few rows: a group of columns a thread, so that a row's loads are one trip; many, which hide each other's trips: fewer waves that wait for each
+  // other's sums (us, one group a thread / two: 1,024 x 2,560 8.4 / 7.8, 2,048 x 2,560 13.5 / 12.8, 4,096 x 4,096 37.3 / 35.0, 600 x 4,096 8.3 /
+  // 7.8; level at 512 rows, and at 2,048 x 5,120 with four groups instead of two 26.1 / 26.8)
+  const bool many = n_rows > 512;
   if (padded <= 1024)
     ARLE_MX_NORM(256, 1);
   else if (padded <= 2048)
-    ARLE_MX_NORM(512, 1);
+    if (many)
+      ARLE_MX_NORM(256, 2);
+    else
+      ARLE_MX_NORM(512, 1);
   else if (padded <= 4096)
-    ARLE_MX_NORM(1024, 1);
+    if (many)
+      ARLE_MX_NORM(512, 2);
+    else
+      ARLE_MX_NORM(1024, 1);
   else if (padded <= 8192)
     ARLE_MX_NORM(1024, 2);
   else
@@ -214,7 +228,7 @@ extern "C" int arle_mx_quantize(const void* x, int code, long long ldx, void* el
   uint8_t* c = static_cast<uint8_t*>(scales);
 #define ARLE_MX_Q(T, BITS, ALIGNED, ROWS)                                                                                        \
   mx_quantize_kernel<T, BITS, ALIGNED, ROWS><<<dim3((rows + ROWS - 1) / ROWS, parts), threads, 0, s>>>(static_cast<const T*>(x), ldx, e, c, \
-                                                                                                       rows, width, padded)
+                                                                                                       rows, width, padded, threads)
 #define ARLE_MX_QR(T, BITS, ALIGNED)          \
   do {                                        \
     if (rows <= 1024)                         \
@@ -255,14 +269,14 @@ extern "C" int arle_mx_values(const void* elements, long long ld, const void* sc
   const uint8_t* c = static_cast<const uint8_t*>(scales);
   if (out_code == kF32) {
     if (bits == kMx8)
-      mx_values_kernel<float, kMx8><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<float*>(out), width);
+      mx_values_kernel<float, kMx8><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<float*>(out), width, threads);
     else
-      mx_values_kernel<float, kMx4><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<float*>(out), width);
+      mx_values_kernel<float, kMx4><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<float*>(out), width, threads);
   } else {
     if (bits == kMx8)
-      mx_values_kernel<bf16, kMx8><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<bf16*>(out), width);
+      mx_values_kernel<bf16, kMx8><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<bf16*>(out), width, threads);
     else
-      mx_values_kernel<bf16, kMx4><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<bf16*>(out), width);
+      mx_values_kernel<bf16, kMx4><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<bf16*>(out), width, threads);
   }
   return launch_status();
 }

@@ -138,7 +138,7 @@ SIGNATURES = {
     "arle_mx_quantize": ("mx_rows", [_p, _i, _ll, _p, _p, _i, _i, _i, _i, _i, _p]),
     "arle_mx_values": ("mx_rows", [_p, _ll, _p, _ll, _i, _p, _i, _i, _i, _p]),
     "arle_mx_add_rmsnorm": ("mx_rows", [_p, _p, _i, _ll, _i, _p, _i, _p, _p, _i, _p, _i, _i, _i, _i, _f, _p]),
-    "arle_mx_gemm": ("mx_gemm", [_i, _i, _i, _p, _ll, _p, _ll, _p, _p, _p, _ll, _ll, _p, _ll, _i, _i, _i, _i, _i, _i, _i, _p]),
+    "arle_mx_gemm": ("mx_gemm", [_i, _i, _i, _p, _ll, _p, _ll, _p, _p, _p, _ll, _p, _ll, _i, _i, _i, _i, _i, _i, _i, _p]),
     "arle_ceiling_read": ("ceilings", [_p, _ll, _i, _p, _p, _p]),
     "arle_ceiling_mfma": ("ceilings", [_i, _i, _i, _i, _p, _p]),
 }

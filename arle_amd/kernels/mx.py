@@ -241,12 +241,12 @@ def add_rmsnorm(residual: torch.Tensor, delta: torch.Tensor | None, weight: torc
 # ------------------------------------------------------------------- products
 
 
-_Weight = collections.namedtuple("_Weight", "tiles scales n k gated n_tiles k_tiles device")
+_Weight = collections.namedtuple("_Weight", "tiles scales n k gated n_tiles k_tiles device pitch")
 
 
 class MXWeight(_Weight):
-    """A weight [n, k] in 4 bits, laid out for the products (see lay_weight).  tiles uint8 [tiles of 16 rows, tiles of 128 k, 64, 16], scales uint8
-    [tiles of 16 rows, groups of 512 k, 64, 4].  gated: n = 2 * ff rows, the gate's and then the up's, held in turns of 16 with both
+    """A weight [n, k] in 4 bits, laid out for the products (see lay_weight).  tiles uint8 [tiles of 128 k, tiles of 16 rows, 64, 16], scales uint8
+    [groups of 512 k, tiles of 16 rows, 64, 4]; both may be the first rows' tiles of a larger weight.  gated: n = 2 * ff rows, the gate's and then the up's, held in turns of 16 with both
     halves padded with zeros to a multiple of 512."""
     __slots__ = ()
 
@@ -258,11 +258,20 @@ class MXWeight(_Weight):
             raise ShapeError(f"a weight has up to {MAX_K} columns and {MAX_WEIGHT} numbers, got [{n}, {k}]")
         k_tiles = padded_width(k) // TILE
         n_tiles = 2 * padded_width(n // 2) // 16 if gated else -(-n // 16)
-        if not (tiles.dtype == torch.uint8 and tuple(tiles.shape) == (n_tiles, k_tiles, 64, 16) and tiles.is_contiguous() and tiles.data_ptr() % 16 == 0
-                and scales.dtype == torch.uint8 and tuple(scales.shape) == (n_tiles, -(-k_tiles // 4), 64, 4) and scales.is_contiguous()
-                and scales.data_ptr() % 16 == 0):
-            raise ShapeError(f"the tiles of a [{n}, {k}] weight are uint8 [{n_tiles}, {k_tiles}, 64, 16], their scales [{n_tiles}, {-(-k_tiles // 4)}, 64, 4]")
-        return tuple.__new__(cls, (tiles, scales, int(n), int(k), bool(gated), n_tiles, k_tiles, device))
+        if not (tiles.dtype == torch.uint8 and tuple(tiles.shape) == (k_tiles, n_tiles, 64, 16) and scales.dtype == torch.uint8
+                and tuple(scales.shape) == (k_tiles // 4, n_tiles, 64, 4)):
+            raise ShapeError(f"the tiles of a [{n}, {k}] weight are uint8 [{k_tiles}, {n_tiles}, 64, 16], their scales [{k_tiles // 4}, {n_tiles}, 64, 4]")
+        pitch = tiles.stride(0) // 1024
+        if (tiles.stride() != (1024 * pitch, 1024, 16, 1) or scales.stride()[1:] != (256, 4, 1) or (k_tiles > 4 and scales.stride(0) != 256 * pitch)
+                or pitch < n_tiles or pitch * k_tiles * 2048 > MAX_WEIGHT or tiles.data_ptr() % 16 or scales.data_ptr() % 16):
+            raise ShapeError("a step's tiles and scales must lie together, start at multiples of 16 bytes and be equally many apart")
+        return tuple.__new__(cls, (tiles, scales, int(n), int(k), bool(gated), n_tiles, k_tiles, device, pitch))
+
+    def first(self, rows: int) -> "MXWeight":
+        """The weight's first `rows` rows, a multiple of 16: a view."""
+        if self.gated or rows % 16 or not 0 < rows <= self.n:
+            raise ShapeError(f"the first {rows} rows of a {'gated' if self.gated else 'plain'} weight of {self.n} are no whole tiles")
+        return MXWeight(self.tiles[:, :rows // 16], self.scales[:, :rows // 16], rows, self.k)
 
     @property
     def nbytes(self) -> int:
@@ -284,8 +293,8 @@ def lay_weight(rows: MXRows, gated: bool = False) -> MXWeight:
         e, s = turns(e), turns(s)
     more = -e.shape[0] % 16
     e, s = torch.nn.functional.pad(e, (0, 0, 0, more)), torch.nn.functional.pad(s, (0, -s.shape[1] % 16, 0, more))
-    tiles = e.reshape(-1, 16, padded // TILE, 4, 16).permute(0, 2, 3, 1, 4).reshape(-1, padded // TILE, 64, 16).contiguous()
-    scales = s.reshape(s.shape[0] // 16, 16, -1, 4, 4).permute(0, 2, 4, 1, 3).reshape(s.shape[0] // 16, -1, 64, 4).contiguous()
+    tiles = e.reshape(-1, 16, padded // TILE, 4, 16).permute(2, 0, 3, 1, 4).reshape(padded // TILE, -1, 64, 16).contiguous()
+    scales = s.reshape(s.shape[0] // 16, 16, -1, 4, 4).permute(2, 0, 4, 1, 3).reshape(padded // 512, -1, 64, 4).contiguous()
     return MXWeight(tiles, scales, n, rows.width, gated)
 
 
@@ -392,7 +401,7 @@ def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partia
     if code is None:
         raise ShapeError("products come in float32 or bfloat16")
     elements, held, _, _, M, _, bits, _ = x
-    tiles, tile_scales, N, _, _, n_tiles, k_tiles, _ = w
+    tiles, tile_scales, N, _, _, n_tiles, k_tiles, _, pitch = w
     on = _DEVICES.get(device) or _device(device)
     if M == 0:
         return _empty(0, N, dtype=out_dtype, device=on)
@@ -404,7 +413,7 @@ def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partia
     parts = splits > 1
     out = _empty(splits, M, N, dtype=torch.float32, device=on) if parts else _empty(M, N, dtype=out_dtype, device=on)
     _call("arle_mx_gemm", bits, _EPI_F32 if parts else code, variant, elements.data_ptr(), elements.stride(0), held.data_ptr(), held.stride(0),
-          tiles.data_ptr(), tile_scales.data_ptr(), out.data_ptr(), N, M * N, 0, 0, M, N, n_tiles, k_tiles, splits, per_split, N % 8 == 0, _stream(device))
+          tiles.data_ptr(), tile_scales.data_ptr(), out.data_ptr(), N, 0, 0, M, N, n_tiles, k_tiles, pitch, splits, per_split, _stream(device))
     if parts and not partials_ok:
         return ops.sum_partials(out, out_dtype)
     return out
@@ -416,7 +425,7 @@ def gate_up_act(x: MXRows, w: MXWeight, form: str = "mxfp8", *, variant: int | N
     device = _checked(x, w, True)
     out_bits = BITS.get(form) or _bits(form)
     elements, held, _, _, M, _, bits, _ = x
-    tiles, tile_scales, n, _, _, n_tiles, k_tiles, _ = w
+    tiles, tile_scales, n, _, _, n_tiles, k_tiles, _, pitch = w
     out = _new_rows(M, n // 2, form, out_bits, device)
     if M == 0:
         return out
@@ -428,6 +437,6 @@ def gate_up_act(x: MXRows, w: MXWeight, form: str = "mxfp8", *, variant: int | N
         per_split = _per_split(M, k_tiles, bits, variant, 1)
     padded = out[5]
     _call("arle_mx_gemm", bits, _EPI_GATE[form], variant, elements.data_ptr(), elements.stride(0), held.data_ptr(), held.stride(0), tiles.data_ptr(),
-          tile_scales.data_ptr(), out[0].data_ptr(), padded * out_bits // 8, 0, out[1].data_ptr(), padded // BLOCK, M, 16 * n_tiles, n_tiles, k_tiles, 1,
-          per_split, True, _stream(device))
+          tile_scales.data_ptr(), out[0].data_ptr(), padded * out_bits // 8, out[1].data_ptr(), padded // BLOCK, M, 16 * n_tiles, n_tiles, k_tiles, pitch, 1,
+          per_split, _stream(device))
     return out

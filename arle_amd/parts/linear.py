@@ -112,11 +112,9 @@ class MXLinear:
 
     def first(self, rows: int) -> "MXLinear":
         """The projection to the first `rows` outputs (a multiple of 16), no copy."""
-        if rows % 16 or self.held.gated:
-            raise ValueError("part of a weight is whole operand tiles of a plain one")
         part = object.__new__(MXLinear)
         part.out_features, part.in_features, part.row_form = rows, self.in_features, self.row_form
-        part.held = mx.MXWeight(self.held.tiles[:rows // 16], self.held.scales[:rows // 16], rows, self.in_features)
+        part.held = self.held.first(rows)
         return part
 
     def rows(self, x) -> mx.MXRows:

@@ -44,17 +44,17 @@ def test_weight_tiles(no_gpu, n, k):
     w = mx.lay_weight(rows)
     assert (w.n, w.k, w.gated) == (n, k, False)
     codes, scales = plain.unpack(rows)
-    for t in range(w.tiles.shape[0]):
-        for st in range(w.tiles.shape[1]):
+    for t in range(w.tiles.shape[1]):
+        for st in range(w.tiles.shape[0]):
             for lane in range(64):
                 g, i = divmod(lane, 16)
                 row = 16 * t + i
-                piece = w.tiles[t, st, lane]
+                piece = w.tiles[st, t, lane]
                 got = torch.stack([piece & 15, piece >> 4], dim=-1).flatten()
                 at = 128 * st + 32 * g
                 want = codes[row, at:at + 32] if row < n else torch.zeros(32, dtype=torch.uint8)
                 assert torch.equal(got, want)
-                assert w.scales[t, st // 4, lane, st % 4] == (scales[row, at // 32] if row < n else 0)
+                assert w.scales[st // 4, t, lane, st % 4] == (scales[row, at // 32] if row < n else 0)
 
 
 @pytest.mark.parametrize("ff", [1, 16, 100, 256, 300])
@@ -62,11 +62,11 @@ def test_gated_weight_is_turns_of_sixteen(no_gpu, ff):
     e, s, rows = _rows(2 * ff, 64, "mxfp4")
     w = mx.lay_weight(rows, gated=True)
     padded = -(-ff // 512) * 512
-    assert w.n == 2 * ff and w.tiles.shape[0] == 2 * padded // 16
+    assert w.n == 2 * ff and w.tiles.shape[1] == 2 * padded // 16
     codes, _ = plain.unpack(rows)
     for c in range(0, padded, 7):
         for which in (0, 1):
-            piece = w.tiles[2 * (c // 16) + which, 0, c % 16]
+            piece = w.tiles[0, 2 * (c // 16) + which, c % 16]
             got = torch.stack([piece & 15, piece >> 4], dim=-1).flatten()
             assert torch.equal(got, codes[which * ff + c, :32] if c < ff else torch.zeros(32, dtype=torch.uint8))
 
@@ -151,8 +151,11 @@ def test_refused_products(no_gpu):
         lambda: mx.gate_up_act(x, wg, "fp4"),
         lambda: mx.gemm(_rows(3, 299)[2], w),
         lambda: mx.gemm(x, w, torch.float16),
-        lambda: mx.gemm(x, mx.MXWeight(w.tiles[:1], w.scales, 40, 300)),
+        lambda: mx.gemm(x, mx.MXWeight(w.tiles[:, :1], w.scales, 40, 300)),
         lambda: mx.gemm(x, mx.MXWeight(w.tiles, w.scales, 60, 300)),
+        lambda: mx.MXWeight(w.tiles[:, :2], w.scales[:, :2].contiguous()[:, :, :32], 32, 300),
+        lambda: mx.MXWeight(w.tiles.transpose(2, 3).contiguous().transpose(2, 3), w.scales, 40, 300),
+        lambda: w.first(24), lambda: w.first(48), lambda: w.first(0), lambda: wg.first(16),
         lambda: mx.gemm(_rows(17, 300)[2], w, variant=0),                # more rows than the kernel holds
         lambda: mx.gemm(x, w, variant=20),
         lambda: mx.gate_up_act(x, wg, variant=7),

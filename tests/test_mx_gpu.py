@@ -236,6 +236,17 @@ def test_strided_rows_and_slices():
     assert torch.equal(mx.values(apart), mx.values(x))
 
 
+@pytest.mark.parametrize("variant", sorted(VARIANT_ROWS))
+@pytest.mark.parametrize("K", [200, 1100])
+def test_the_first_rows_of_a_weight(variant, K):
+    """Tiles of a larger weight: a step's tiles lie further apart than there are."""
+    x = mx.quantize(torch.randn(13, K, generator=_g(1)).to(DEV))
+    w = mx.lay_weight(mx.quantize(torch.randn(600, K, generator=_g(2)).to(DEV), "mxfp4"))
+    whole = mx.gemm(x, w, torch.float32, variant=variant)
+    for n in (16, 48, 400):
+        assert torch.equal(mx.gemm(x, w.first(n), torch.float32, variant=variant), whole[:, :n])
+
+
 def test_every_kernel_of_few_or_many_rows_gives_the_same_row_whatever_stands_beside_it():
     x = mx.quantize(torch.randn(300, 700, generator=_g(1)).to(DEV))
     w = mx.lay_weight(mx.quantize(torch.randn(90, 700, generator=_g(2)).to(DEV), "mxfp4"))
