@@ -59,18 +59,16 @@ def _same_device(held: int) -> int:
 _functions: dict = {}
 
 
-def _call(name: str, *args) -> None:
-    """lib.call with the function found once."""
-    fn = _functions.get(name)
-    if fn is None:
-        fn = _functions[name] = lib.function(name)
-    status = fn(*args)
-    if status:
-        raise lib.KernelError(f"{name} failed with HIP error {status}")
+def _function(name: str):
+    fn = _functions[name] = lib.function(name)
+    return fn
 
 
-def _stream(device: int) -> int:
-    return ops._raw_stream(device) if ops._raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+def _failed(name: str, status: int) -> None:
+    raise lib.KernelError(f"{name} failed with HIP error {status}")
+
+
+_stream = ops._raw_stream or (lambda device: torch.cuda.current_stream(device).cuda_stream)      # handle of the current stream of a device
 
 
 def _bits(form: str) -> int:
@@ -178,7 +176,10 @@ def quantize(x: torch.Tensor, form: str = "mxfp8") -> MXRows:
     if T:
         at = x.data_ptr()
         aligned = K % 8 == 0 and stride % 4 == 0 and at % (16 if code == F32 else 8) == 0
-        _call("arle_mx_quantize", at, code, stride, out[0].data_ptr(), out[1].data_ptr(), bits, T, K, out[5], aligned, _stream(device))
+        status = (_functions.get("arle_mx_quantize") or _function("arle_mx_quantize"))(
+            at, code, stride, out[0].data_ptr(), out[1].data_ptr(), bits, T, K, out[5], aligned, _stream(device))
+        if status:
+            _failed("arle_mx_quantize", status)
     return out
 
 
@@ -191,8 +192,11 @@ def values(x: MXRows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         raise ShapeError("values come in float32 or bfloat16")
     out = torch.empty((x.rows, x.width), dtype=dtype, device=_device(device))
     if x.rows:
-        _call("arle_mx_values", x.elements.data_ptr(), x.elements.stride(0), x.scales.data_ptr(), x.scales.stride(0), x.bits, out.data_ptr(),
-                 _CODES[dtype], x.rows, x.width, _stream(device))
+        status = (_functions.get("arle_mx_values") or _function("arle_mx_values"))(
+            x.elements.data_ptr(), x.elements.stride(0), x.scales.data_ptr(), x.scales.stride(0), x.bits, out.data_ptr(),
+            _CODES[dtype], x.rows, x.width, _stream(device))
+        if status:
+            _failed("arle_mx_values", status)
     return out
 
 
@@ -207,10 +211,9 @@ def add_rmsnorm(residual: torch.Tensor, delta: torch.Tensor | None, weight: torc
     if (device < 0 or device != _current() or weight.get_device() != device or (delta is not None and delta.get_device() != device)
             or (rows is not None and rows.get_device() != device)):
         _here(residual, delta, weight, rows)
-    shape = residual.shape
-    if residual.dtype != torch.float32 or len(shape) != 2 or not residual.is_contiguous():
+    if residual.dtype is not torch.float32 or residual.dim() != 2 or not residual.is_contiguous():
         raise ShapeError("residual must be contiguous float32 [T, H]")
-    T, width = shape
+    T, width = residual.shape
     if not 0 < width <= MAX_WIDTH:
         raise ShapeError(f"a norm's rows have 1 to {MAX_WIDTH} columns, got {width}")
     at, w_at, w_code = residual.data_ptr(), weight.data_ptr(), _CODES.get(weight.dtype)
@@ -219,10 +222,14 @@ def add_rmsnorm(residual: torch.Tensor, delta: torch.Tensor | None, weight: torc
     aligned = width % 4 == 0 and at % 16 == 0 and w_at % (16 if w_code == F32 else 8) == 0
     n_delta = delta_at = delta_code = 0
     if delta is not None:
-        n_delta, of, delta_code = 1, delta.shape, _CODES.get(delta.dtype)
-        if len(of) == 3:
-            n_delta, of = of[0], of[1:]
-        if of != shape or delta_code is None or n_delta < 1 or not delta.is_contiguous():
+        n_delta, delta_code, dims = 1, _CODES.get(delta.dtype), delta.dim()
+        if dims == 3:
+            n_delta, rows_of, width_of = delta.shape
+        elif dims == 2:
+            rows_of, width_of = delta.shape
+        else:
+            rows_of = width_of = -1
+        if rows_of != T or width_of != width or delta_code is None or n_delta < 1 or not delta.is_contiguous():
             raise ShapeError("delta must match the residual ([T, H] or a stack [S, T, H]) in float32 or bfloat16")
         delta_at = delta.data_ptr()
         aligned = aligned and delta_at % (16 if delta_code == F32 else 8) == 0
@@ -233,8 +240,11 @@ def add_rmsnorm(residual: torch.Tensor, delta: torch.Tensor | None, weight: torc
         n_rows = rows.numel()
     out = _new_rows(n_rows, width, form, bits, device)
     if n_rows:
-        _call("arle_mx_add_rmsnorm", at, delta_at, n_delta, T * width, delta_code, w_at, w_code, out[0].data_ptr(), out[1].data_ptr(), bits,
-              _ptr(rows), n_rows, width, out[5], aligned, eps, _stream(device))
+        status = (_functions.get("arle_mx_add_rmsnorm") or _function("arle_mx_add_rmsnorm"))(
+            at, delta_at, n_delta, T * width, delta_code, w_at, w_code, out[0].data_ptr(), out[1].data_ptr(), bits,
+            _ptr(rows), n_rows, width, out[5], aligned, eps, _stream(device))
+        if status:
+            _failed("arle_mx_add_rmsnorm", status)
     return out
 
 
@@ -412,8 +422,11 @@ def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partia
         per_split = _per_split(M, k_tiles, bits, variant, splits)
     parts = splits > 1
     out = _empty(splits, M, N, dtype=torch.float32, device=on) if parts else _empty(M, N, dtype=out_dtype, device=on)
-    _call("arle_mx_gemm", bits, _EPI_F32 if parts else code, variant, elements.data_ptr(), elements.stride(0), held.data_ptr(), held.stride(0),
-          tiles.data_ptr(), tile_scales.data_ptr(), out.data_ptr(), N, 0, 0, M, N, n_tiles, k_tiles, pitch, splits, per_split, _stream(device))
+    status = (_functions.get("arle_mx_gemm") or _function("arle_mx_gemm"))(
+        bits, _EPI_F32 if parts else code, variant, elements.data_ptr(), elements.stride(0), held.data_ptr(), held.stride(0),
+            tiles.data_ptr(), tile_scales.data_ptr(), out.data_ptr(), N, 0, 0, M, N, n_tiles, k_tiles, pitch, splits, per_split, _stream(device))
+    if status:
+        _failed("arle_mx_gemm", status)
     if parts and not partials_ok:
         return ops.sum_partials(out, out_dtype)
     return out
@@ -436,7 +449,10 @@ def gate_up_act(x: MXRows, w: MXWeight, form: str = "mxfp8", *, variant: int | N
             raise ShapeError(f"variant {variant} makes no blocks")
         per_split = _per_split(M, k_tiles, bits, variant, 1)
     padded = out[5]
-    _call("arle_mx_gemm", bits, _EPI_GATE[form], variant, elements.data_ptr(), elements.stride(0), held.data_ptr(), held.stride(0), tiles.data_ptr(),
-          tile_scales.data_ptr(), out[0].data_ptr(), padded * out_bits // 8, out[1].data_ptr(), padded // BLOCK, M, 16 * n_tiles, n_tiles, k_tiles, pitch, 1,
-          per_split, _stream(device))
+    status = (_functions.get("arle_mx_gemm") or _function("arle_mx_gemm"))(
+        bits, _EPI_GATE[form], variant, elements.data_ptr(), elements.stride(0), held.data_ptr(), held.stride(0), tiles.data_ptr(),
+            tile_scales.data_ptr(), out[0].data_ptr(), padded * out_bits // 8, out[1].data_ptr(), padded // BLOCK, M, 16 * n_tiles, n_tiles, k_tiles, pitch, 1,
+            per_split, _stream(device))
+    if status:
+        _failed("arle_mx_gemm", status)
     return out

@@ -13,10 +13,11 @@ def no_gpu(monkeypatch):
     monkeypatch.setattr(mx, "_current", lambda: 0)
     monkeypatch.setattr(mx, "_DEVICES", {d: torch.device("cpu") for d in (-1, 0)})
 
-    def call(name, *args):
-        raise AssertionError(f"{name} was launched")
+    class Functions(dict):
+        def get(self, name):
+            raise AssertionError(f"{name} was launched")
 
-    monkeypatch.setattr(mx, "_call", call)
+    monkeypatch.setattr(mx, "_functions", Functions())
 
 
 def _rows(T, width, form="mxfp8", seed=0):
@@ -124,6 +125,8 @@ def test_refused_norms(no_gpu):
         lambda: mx.add_rmsnorm(res, res[:2], w, 1e-6),
         lambda: mx.add_rmsnorm(res, torch.zeros(0, 3, 64), w, 1e-6),
         lambda: mx.add_rmsnorm(res, res.half(), w, 1e-6),
+        lambda: mx.add_rmsnorm(res, torch.zeros(64), w, 1e-6),
+        lambda: mx.add_rmsnorm(res, torch.zeros(1, 1, 3, 64), w, 1e-6),
         lambda: mx.add_rmsnorm(res, None, w[:63], 1e-6),
         lambda: mx.add_rmsnorm(res, None, w.half(), 1e-6),
         lambda: mx.add_rmsnorm(res, None, w, 1e-6, "fp8"),
