@@ -187,11 +187,12 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
   constexpr int kRowBytes = 16 * BITS, kPieces = kRowBytes / 16, kRowsALoad = 64 / kPieces;
   constexpr int kXBytes = kRows * kRowBytes, kStage = kXBytes + kTiles * 1024;
   constexpr int kXScales = (kRows < 64 ? 64 : kRows) * 16, kScales = kXScales + kTiles * 256;   // of a round
-  constexpr int XD = kXBytes / 1024 / kWaves, WD = kTiles / kWaves, kBatch = XD + WD;   // loads of a wave and step
+  constexpr int XD = kXBytes / 1024 / kWaves, WD = (kTiles + kWaves - 1) / kWaves, kBatch = XD + WD;   // loads of a wave and step
   // operands are read kAhead groups before their products (us, one / two: 256 x 256 at gate|up of 4,096 x 12,288 x 4,096 307 / 302, 128 x 192 at
   // 2,048 x 2,560 x 9,728 45.4 / 46.2)
   constexpr int kGroups = 2 * MT, kAhead = MT >= 4 ? 2 : 1, kRing = kAhead == 1 ? 2 : 4;
-  static_assert(XD * kWaves * 1024 == kXBytes && WD * kWaves == kTiles && kTiles % 4 == 0, "whole loads a wave");
+  static_assert(XD * kWaves * 1024 == kXBytes && kTiles % 4 == 0, "whole loads");
+  static_assert((STAGES - 2) * kBatch <= 63, "loads on their way are counted in six bits");
   static_assert(STAGES >= 2 && STAGES <= 8, "a step's batch is sent STAGES - 1 steps ahead; a ninth would overtake a round's scales");
   extern __shared__ __align__(16) unsigned char lds[];
   unsigned char* const lds_scales = lds + STAGES * kStage;
@@ -219,8 +220,13 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
     x_off[p] = static_cast<uint32_t>(min(row, a.M - 1 - m0)) * static_cast<uint32_t>(a.ldx) + slot(row, lane % kPieces) * 16;
   }
   const uint8_t* w0[WD];
+  int w_to[WD];
 #pragma unroll
-  for (int q = 0; q < WD; ++q) w0[q] = a.w + static_cast<int64_t>(min(tile0 + WD * wave + q, a.n_tiles - 1)) * 1024;
+  for (int q = 0; q < WD; ++q) {      // a load too many is the last one again
+    const int piece = min(WD * wave + q, kTiles - 1);
+    w0[q] = a.w + static_cast<int64_t>(min(tile0 + piece, a.n_tiles - 1)) * 1024;
+    w_to[q] = kXBytes + piece * 1024;
+  }
   // a round's scales are kilobytes too: 64 rows of X or four tiles of W; which is which is a matter of addresses, as a branch in the loop
   // would part it into pieces between which the compiler moves products; a load too many is the last one again
   constexpr int kXItems = kXScales / 1024, kItems = kXItems + kTiles / 4, SD = (kItems + kWaves - 1) / kWaves;
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
     if (i < XD)
       load_to_lds_16(x0 + abs * kRowBytes, x_off[i], to + (XD * wave + i) * 1024);
     else
-      load_to_lds_16(w0[i - XD] + abs * (static_cast<int64_t>(a.pitch) * 1024), lane * 16, to + kXBytes + (WD * wave + i - XD) * 1024);
+      load_to_lds_16(w0[i - XD] + abs * (static_cast<int64_t>(a.pitch) * 1024), lane * 16, to + w_to[i - XD]);
   };
 
   mx_f32x16 acc[MT][TN];
@@ -491,6 +497,7 @@ int mx_launch(int variant, const MxArgs& a, int splits, hipStream_t s) {
     case 5: return mx_tiles_launch<BITS, EPI, 2, 2, 2, 4, BITS == kMx8 ? 4 : 5, 2>(a, splits, s);
     case 6: return mx_tiles_launch<BITS, EPI, 4, 2, 2, 4, BITS == kMx8 ? 3 : 4, 2>(a, splits, s);
     case 7: if constexpr (!kGate) return mx_tiles_launch<BITS, EPI, 2, 3, 2, 2, 5, 1>(a, splits, s); else break;
+    case 8: if constexpr (!kGate) return mx_tiles_launch<BITS, EPI, 2, 3, 4, 2, BITS == kMx8 ? 3 : 5, 2>(a, splits, s); else break;
   }
   return static_cast<int>(hipErrorInvalidValue);
 }

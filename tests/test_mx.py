@@ -161,7 +161,7 @@ def test_refused_products(no_gpu):
         lambda: w.first(24), lambda: w.first(48), lambda: w.first(0), lambda: wg.first(16),
         lambda: mx.gemm(_rows(17, 300)[2], w, variant=0),                # more rows than the kernel holds
         lambda: mx.gemm(x, w, variant=20),
-        lambda: mx.gate_up_act(x, wg, variant=7),
+        lambda: mx.gate_up_act(x, wg, variant=8),
         lambda: mx.gate_up_act(x, wg, variant=0),
         lambda: mx.gemm(x, w, variant=0, splits=5),                      # four steps of 128
         lambda: mx.gemm(_rows(3, 300, "mxfp4")[2], w, variant=3, splits=2),   # one round of 512
