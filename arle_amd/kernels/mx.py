@@ -102,9 +102,12 @@ class MXRows(_Rows):
                 and tuple(s.shape) == (e.shape[0], padded // BLOCK)):
             raise ShapeError(f"{form} rows of {width} are {_ELEMENTS[form]} [T, {padded * bits // 8}] with scales {_SCALES} [T, {padded // BLOCK}], got "
                              f"{e.dtype} {tuple(e.shape)} with {s.dtype} {tuple(s.shape)}")
-        if e.stride(1) != 1 or s.stride(1) != 1 or e.data_ptr() % 16 or s.data_ptr() % 16 or (e.shape[0] > 1 and (e.stride(0) % 16 or s.stride(0) % 16 or e.stride(0) > 2 * MAX_K)):
-            raise ShapeError("rows of elements and scales must lie together and start at multiples of 16 bytes")
+        if e.stride(1) != 1 or s.stride(1) != 1 or e.data_ptr() % 16 or s.data_ptr() % 16 or (e.shape[0] > 1 and (e.stride(0) % 16 or s.stride(0) % 16 or max(e.stride(0), s.stride(0)) > 2 * MAX_K)):
+            raise ShapeError(f"rows of elements and scales must lie together and start at multiples of 16 bytes, up to {2 * MAX_K} apart")
         return tuple.__new__(cls, (e, s, int(width), form, e.shape[0], padded, bits, device))
+
+    def __getnewargs__(self):      # of a copy: what it is made from, which is checked again
+        return self[:4]
 
     def part(self, start: int, stop: int) -> "MXRows":
         """Rows start .. stop - 1, a view."""
@@ -277,6 +280,9 @@ class MXWeight(_Weight):
             raise ShapeError("a step's tiles and scales must lie together, start at multiples of 16 bytes and be equally many apart")
         return tuple.__new__(cls, (tiles, scales, int(n), int(k), bool(gated), n_tiles, k_tiles, device, pitch))
 
+    def __getnewargs__(self):
+        return self[:5]
+
     def first(self, rows: int) -> "MXWeight":
         """The weight's first `rows` rows, a multiple of 16: a view."""
         if self.gated or rows % 16 or not 0 < rows <= self.n:
@@ -444,7 +450,7 @@ def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partia
 
 def gate_up_act(x: MXRows, w: MXWeight, form: str = "mxfp8", *, variant: int | None = None) -> MXRows:
     """silu(x . gate^T) * (x . up^T) in blocks, [T, ff] from a weight laid out with gated=True: the rows of the second half's product,
-    made from the 32-bit sums in one kernel."""
+    made from the 32-bit sums in one kernel.  (A row with a block that is no number is none throughout, its padding too.)"""
     device = _checked(x, w, True)
     out_bits = BITS.get(form) or _bits(form)
     elements, held, _, _, M, _, bits, _ = x

@@ -1,4 +1,6 @@
 """Microscaled rows and weights on the host: layouts of weights, and the calls that the entry points refuse before anything is launched."""
+import copy
+
 import pytest
 import torch
 
@@ -110,11 +112,21 @@ def test_refused_rows(no_gpu):
         lambda: mx.MXRows(_e8(2, 512), _s(2, 16).view(torch.uint8), 512, "mxfp8"),
         lambda: mx.MXRows(_e8(2, 512), _s(2, 16), 0, "mxfp8"),
         lambda: mx.MXRows(_e8(2, 512), _s(2, 32), 1024, "mxfp4"),
+        lambda: mx.MXRows(_e8(2, 2**23 + 16)[:, :512], _s(2, 16), 512, "mxfp8"),      # rows further apart than offsets of 32 bits reach over 256 of them
+        lambda: mx.MXRows(_e8(2, 512), _s(2, 2**23 + 16)[:, :16], 512, "mxfp8"),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(ops.ShapeError):
             call()
             pytest.fail(f"call {i} passed")
+
+
+@pytest.mark.parametrize("copied", [copy.copy, copy.deepcopy])
+def test_rows_and_weights_can_be_copied(no_gpu, copied):
+    rows, weight = _rows(3, 600)[2], mx.lay_weight(_rows(34, 600, "mxfp4")[2], gated=True)
+    for a in (rows, weight):
+        b = copied(a)
+        assert type(b) is type(a) and all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a[:2], b[:2])) and a[2:] == b[2:]
 
 
 def test_refused_norms(no_gpu):

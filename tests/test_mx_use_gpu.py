@@ -1,0 +1,188 @@
+"""The microscaled kernels as programs use them: one behind the other, captured, on several streams and threads, with numbers that are none,
+and at sizes past 32 bits."""
+import threading
+
+import pytest
+import torch
+
+import plain_mx as plain
+import tiny
+from arle_amd.engine import Engine, StepEntry
+from arle_amd.kernels import mx
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+FORMS = ["mxfp8", "mxfp4"]
+
+
+def _g(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+class _FeedForward:
+    """Norm, gated first half, second half and the norm behind it, which adds the stack that a product may leave."""
+
+    def __init__(self, H, ff, form, seed):
+        n = lambda *shape: torch.randn(*shape, generator=_g(seed + len(shape) + shape[0]))
+        self.form = form
+        self.plain = [(1 + 0.1 * n(H)).double(), n(2 * ff, H).double() * H**-0.5, n(H, ff).double() * ff**-0.5]
+        self.norm = self.plain[0].float().to(DEV)
+        self.gate_up = mx.lay_weight(mx.quantize(self.plain[1].float().to(DEV), "mxfp4"), gated=True)
+        self.down = mx.lay_weight(mx.quantize(self.plain[2].float().to(DEV), "mxfp4"))
+
+    def __call__(self, residual, x):
+        rows = mx.add_rmsnorm(residual, x, self.norm, 1e-6, self.form)
+        stack = mx.gemm(mx.gate_up_act(rows, self.gate_up, self.form), self.down, partials_ok=True)
+        return mx.values(mx.add_rmsnorm(residual, stack, self.norm, 1e-6, self.form))
+
+    def in_64_bits(self, residual, x, rounded):
+        norm, gate_up, down = self.plain
+        held = lambda w: plain.round_rows(w, "mxfp4")
+        rows = (lambda v: plain.round_rows(v, self.form)) if rounded else (lambda v: v)
+        h, y = plain.norm(residual, x, norm, 1e-6)
+        d = rows(plain.gated(rows(y), held(gate_up))) @ held(down).T
+        h, y = plain.norm(h, d, norm, 1e-6)
+        return h, rows(y)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("T,H,ff", [(1, 260, 700), (7, 1100, 300), (40, 512, 1530)])
+def test_one_behind_the_other(form, T, H, ff):
+    """Off from the same blocks in 64 bits by less than rounding every number to its element is off from not rounding: the two differ
+    where 32 bits, or a product's bfloat16, put a number on the other side of a border between two elements."""
+    part = _FeedForward(H, ff, form, 3)
+    residual, x = torch.randn(T, H, generator=_g(1)), torch.randn(T, H, generator=_g(2)).bfloat16()
+    h, y = part.in_64_bits(residual, x, True)
+    h0, y0 = part.in_64_bits(residual, x, False)
+    r = residual.to(DEV)
+    got = part(r, x.to(DEV)).cpu().double()
+    assert (r.cpu().double() - h).norm() <= (h - h0).norm() and (got - y).norm() <= (y - y0).norm()
+
+
+def test_captured_at_the_first_call_and_replayed():
+    """Two graphs of the same program, replayed several times in turn on two streams with new inputs, eager calls and synchronisations
+    between; each keeps its own results."""
+    parts = [_FeedForward(520, 300, form, 5) for form in FORMS]
+    w = mx.lay_weight(mx.quantize(torch.randn(600, 520, generator=_g(7)).to(DEV), "mxfp4"))
+    make = lambda: (torch.zeros(16, 520, device=DEV), torch.zeros(16, 520, dtype=torch.bfloat16, device=DEV))
+
+    def program(residual, x):
+        q = mx.quantize(x, "mxfp8")
+        outs = [mx.gemm(q, w, torch.float32, variant=v) for v in range(9)] + [p(residual, x) for p in parts]
+        return outs + [mx.values(q), mx.gemm(q, w, variant=2, splits=2)]
+
+    torch.cuda.synchronize()
+    held = []
+    for _ in range(2):
+        inputs = make()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = program(*inputs)
+        held.append((inputs, graph, outs))
+    streams = [torch.cuda.Stream() for _ in held]
+    for turn in range(4):
+        given = [(torch.randn(16, 520, generator=_g(10 * turn + i)), torch.randn(16, 520, generator=_g(10 * turn + i + 5)).bfloat16()) for i in range(2)]
+        for (inputs, _, _), new in zip(held, given):
+            for t, v in zip(inputs, new):
+                t.copy_(v)
+        torch.cuda.synchronize()
+        for (_, graph, _), s in zip(held, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (inputs, _, outs), (residual, x) in zip(held, given):
+            r = residual.to(DEV)
+            want = program(r, x.to(DEV))
+            assert torch.equal(inputs[0], r)
+            for i, (a, b) in enumerate(zip(outs, want)):
+                assert torch.equal(a, b), (turn, i)
+
+
+def test_threads_with_streams_of_their_own():
+    part = _FeedForward(300, 200, "mxfp8", 9)
+    given = [(torch.randn(5 + i, 300, generator=_g(i)).to(DEV), torch.randn(5 + i, 300, generator=_g(i + 9)).to(DEV)) for i in range(4)]
+    want = [part(r.clone(), x) for r, x in given]
+    torch.cuda.synchronize()
+    off, done = [], []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(50):
+                if not torch.equal(part(given[i][0].clone(), given[i][1]), want[i]):
+                    off.append(i)
+            s.synchronize()
+        done.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not off and len(done) == 4
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_numbers_that_are_none(form):
+    """A block that is no number makes its row's results none, or its column's, and nobody else's; sums past the type are infinite."""
+    M, N, K = 70, 150, 300
+    x, w = torch.randn(M, K, generator=_g(1)), torch.randn(N, K, generator=_g(2))
+    clean_x, clean_w = x.clone(), w.clone()
+    x[3, 40], x[69, 299], w[10, 0], w[149, 64] = float("nan"), float("inf"), float("-inf"), float("nan")
+    lay = lambda t, **kw: mx.lay_weight(mx.quantize(t.to(DEV), "mxfp4"), **kw)
+    q, clean = mx.quantize(x.to(DEV), form), mx.quantize(clean_x.to(DEV), form)
+    bad_rows, bad_columns = torch.zeros(M, dtype=torch.bool, device=DEV), torch.zeros(N, dtype=torch.bool, device=DEV)
+    bad_rows[[3, 69]], bad_columns[[10, 149]] = True, True
+    bad = bad_rows[:, None] | bad_columns[None]
+    for variant in range(2, 9):
+        want = mx.gemm(clean, lay(clean_w), torch.float32, variant=variant)
+        got = mx.gemm(q, lay(w), torch.float32, variant=variant)
+        assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], want[~bad]), variant
+    rows = q.part(0, 9), clean.part(0, 9)
+    for variant in (0, 1):
+        got, want = mx.gemm(rows[0], lay(w), torch.float32, variant=variant), mx.gemm(rows[1], lay(clean_w), torch.float32, variant=variant)
+        assert torch.equal(got.isnan(), bad[:9]) and torch.equal(got[~bad[:9]], want[~bad[:9]]), variant
+    # gated: column 10 of the gate's half and 149 - 75 = 74 of the up's; each one's block of 32 is none
+    blocks = torch.zeros(M, 3, dtype=torch.bool, device=DEV)
+    blocks[:, [0, 2]] = True
+    blocks[bad_rows] = True
+    for variant in (3, 4, 5, 6):
+        e, s = plain.unpack(mx.gate_up_act(q, lay(w, gated=True), form, variant=variant))
+        ce, cs = plain.unpack(mx.gate_up_act(clean, lay(clean_w, gated=True), form, variant=variant))
+        b = blocks.cpu()
+        assert torch.equal(s[:, :3] == 255, b) and torch.equal(s[:, :3][~b], cs[:, :3][~b]), variant
+        wide = b.repeat_interleave(32, 1)[:, :75]
+        assert not e[:, :75][wide].any() and torch.equal(e[:, :75][~wide], ce[:, :75][~wide]), variant
+    # 2^100 times 2^100; a column without weights stays zero
+    huge = mx.quantize(torch.full((20, 64), 2.0**100, device=DEV), form)
+    big = torch.full((40, 64), 2.0**100)
+    big[1] = 0
+    for variant in (2, 4, 8):
+        got = mx.gemm(huge, lay(big), torch.float32, variant=variant)
+        assert got[:, 1].eq(0).all() and got[:, [0, 2, 39]].isinf().all()
+
+
+def test_results_past_32_bits_of_numbers():
+    M, N = 70001, 32768
+    e = torch.randint(0, 100, (M, 64), generator=_g(1), dtype=torch.uint8)
+    s = torch.randint(120, 130, (M, 2), generator=_g(2), dtype=torch.uint8)
+    x = mx.rows_from_codes(e.to(DEV), s.to(DEV), 64, "mxfp8")
+    w = mx.lay_weight(mx.quantize(torch.randn(N, 64, generator=_g(3)).to(DEV), "mxfp4"))
+    whole = mx.gemm(x, w)
+    assert whole.numel() > 2**31
+    for start in (0, 35000, M - 40):
+        assert torch.equal(whole[start:start + 40], mx.gemm(x.part(start, start + 40), w))
+    del whole
+    wide = torch.randn(1, 8192, generator=_g(4)).to(DEV).bfloat16().expand(280000, 8192).contiguous()
+    wide[-1] = wide[-1] * 3
+    q = mx.quantize(wide)
+    last = mx.quantize(wide[-3:])
+    assert all(torch.equal(a, b) for a, b in zip(plain.unpack(q.part(279997, 280000)), plain.unpack(last)))
+    assert torch.equal(mx.values(q, torch.bfloat16)[-3:], mx.values(last, torch.bfloat16))
+
+
+def test_tuning_leaves_such_projections_alone(tmp_path):
+    """The table of measured products is of products in bfloat16: the head's here."""
+    d = tiny.make_model_dir(tmp_path, "A")
+    engine = Engine.from_folder(d, max_tokens=64, weight_form="mxfp4")
+    engine.tune_products(rows=[1, 8])
+    engine.add_request("x")
+    assert torch.isfinite(engine.step([StepEntry("x", [1, 2, 3], [2])])).all()
