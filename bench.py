@@ -1410,11 +1410,15 @@ def main() -> int:
     for i in range(5):      # eager, captured, then replays until the clocks have settled (the sixth run is as fast as the twentieth)
         prefill_once(("warm", i))
     prefill_s = min(prefill_once(("prefill", i)) for i in range(5))
-    prefill = {"value": round(PROMPT / prefill_s, 1), "tokens": PROMPT, "ms": round(prefill_s * 1e3, 3),
-               "frac": round(prefill_flops(raw, PROMPT) / prefill_s / PEAK_FLOPS[dkey], 4)}
+    prefill = {"value": round(PROMPT / prefill_s, 1), "tokens": PROMPT, "ms": round(prefill_s * 1e3, 3)}
+    held = ""
+    if args.weight_form:
+        held = f", projections in {args.weight_form}, rows in {args.row_form}"
+    else:
+        prefill["frac"] = round(prefill_flops(raw, PROMPT) / prefill_s / PEAK_FLOPS[dkey], 4)
     print(f"[bench] prefill {prefill}", file=sys.stderr, flush=True)
     if args.prefill_only:
-        print(json.dumps({"metric": f"prefill tok/s at {PROMPT} tokens (Qwen3-4B shape, random weights)",
+        print(json.dumps({"metric": f"prefill tok/s at {PROMPT} tokens (Qwen3-4B shape, random weights){held}",
                           "value": prefill["value"], "unit": "tok/s", "n_gpus": 1, "dtype": dkey,
                           "higher_is_better": True, "prefill": prefill}))
         return 0
@@ -1533,7 +1537,8 @@ def main() -> int:
             line["prefill_parts_us"]["timed_step"] = round(prefill["ms"] * 1e3, 1)
             line["decode_parts_us"]["timed_step"] = round(ms_per_step * 1e3, 1)
     if args.weight_form:
-        line["metric"] += f", projections in {args.weight_form}, rows in {args.row_form}"
+        line["metric"] += held
+        line["dtype"] = f"{dkey}, products in {args.row_form} x {args.weight_form}"
         line["config"].update(weight_form=args.weight_form, row_form=args.row_form)
         line.pop("roofline")      # of the bytes of bfloat16 weights
     if args.batch != 8:
