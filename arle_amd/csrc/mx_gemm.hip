@@ -175,10 +175,16 @@ __global__ __launch_bounds__(WAVES* kWave) void mx_gemm_rows_kernel(const MxArgs
 //     barrier stands before its last groups, whose operands are in registers: behind it the next step's stage is there and this
 //     step's is free, and the next step's first operands are read while the last products run.
 //
-// What bounds it (MI355X): 4,096 x 4,096 x 12,288 in 256 x 256, one workgroup a compute unit, takes 135 us, 3.0 PFLOP/s; the same without its
+//   * Workgroups stay (kStays): as many as run at once, each going on to its next tile with the next tile's first steps on their way or there before
+//     its results leave, through the one stage that is free.  (us, a workgroup a tile / staying: gate|up of 4,096 x 12,288 x 4,096 292 / 277, with
+//     X in e2m1 210 / 197, 4,096 x 6,144 x 4,096 79.4 / 75.3 and 59.9 / 55.2, 8,192 x 6,144 x 2,560 100 / 93; with one tile a workgroup, 2,048 x 2,560 x
+//     9,728, 43.3 / 44.1.)  The small tiles' eight stages reach further than the next tile, so theirs have one tile each.
+//
+// What bounds it (MI355X): 4,096 x 4,096 x 12,288 in 256 x 256, one workgroup a compute unit, takes 134 us, 3.1 PFLOP/s; the same without its
 // loads 115, with nothing but its loads 81 (14.5 TB/s from the L2s), the matrix cores are busy 87 % of the time and the clock is down to
-// 1.9 GHz.  Smaller tiles are bound by their loads: 2,048 x 2,560 x 9,728 in 128 x 192 44 us, without loads 34, loads alone 32; 4,096 x 6,144 x
-// 4,096 with X in e2m1, twice the products a second, 64, 50 and 50.  Waves that only load (one or two a workgroup) cannot send fast enough: 45 -> 55 us.
+// 1.9 GHz.  Shorter ones are bound by what a compute unit does at once: 2,048 x 2,560 x 9,728 in 128 x 192 44 us, 42 with every load a hit in the
+// first cache, 38 without loads, 35 without reads of LDS either; 4,096 x 6,144 x 4,096 with X in e2m1 55, 51, 43 and 35.  Waves that only load (one
+// or two a workgroup) cannot send fast enough: 45 -> 55 us.
 template <int BITS, int MT, int TN, int RW, int CW, int STAGES, int WAVES_A_SIMD, int EPI>
 __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_kernel(const MxArgs a) {
   constexpr bool kGate = EPI == kMxGate8 || EPI == kMxGate4;
@@ -190,6 +196,7 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
   constexpr int XD = kXBytes / 1024 / kWaves, WD = (kTiles + kWaves - 1) / kWaves, kBatch = XD + WD;   // loads of a wave and step
   // operands are read kAhead groups before their products (us, one / two: 256 x 256 at gate|up of 4,096 x 12,288 x 4,096 307 / 302, 128 x 192 at
   // 2,048 x 2,560 x 9,728 45.4 / 46.2)
+  constexpr bool kStays = STAGES <= 5;     // a batch is sent at most four steps ahead, which a tile has: to the next one at most
   constexpr int kGroups = 2 * MT, kAhead = MT >= 4 ? 2 : 1, kRing = kAhead == 1 ? 2 : 4;
   static_assert(XD * kWaves * 1024 == kXBytes && kTiles % 4 == 0, "whole loads");
   static_assert((STAGES - 2) * kBatch <= 63, "loads on their way are counted in six bits");
@@ -200,70 +207,78 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
   const int j = lane & 31, h = lane >> 5;
   const int wr = wave / CW, wc = wave % CW;
 
-  // workgroup -> (row block, column block): an XCD's workgroups one behind the other, eight row blocks of a column block side by side
+  // A launch's places, in turns of gridDim.x, are tiles (row block, column block): an XCD's one behind the other, eight row blocks of a column
+  // block side by side.  The last blocks are moved in front so that they end where the rows and columns end (what two workgroups own then they
+  // both write, the same): so the places in memory of a tile's loads hang on the tile by its first row and column only, which are scalars, and
+  // a workgroup goes on to its next tile without a branch.
   const int total = a.m_blocks * a.n_blocks, per_xcd = (total + 7) / 8;
-  const int id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  const auto tile_at = [&](int place) { return place < 8 * per_xcd ? (place & 7) * per_xcd + (place >> 3) : total; };
+  int place = blockIdx.x, id = tile_at(place);
   if (id >= total) return;   // the whole workgroup
-  const int group = id / (8 * a.n_blocks), first = group * 8, rows_here = min(8, a.m_blocks - first), in = id - group * 8 * a.n_blocks;
-  const int mb = first + in % rows_here, nb = in / rows_here;
-  const int m0 = mb * kRows, tile0 = nb * kTiles, n0 = (nb * CW + wc) * (32 * TN);
   const int k_tiles = a.k_tiles, rounds = k_tiles / 4;
   const int r_begin = blockIdx.y * a.per_split, n_rounds = min(a.per_split, rounds - r_begin), n_steps = 4 * n_rounds;
 
   // what the wave fetches: XD kilobytes of rows of X, tiles WD wave .. of W, 64 rows' scales (the first waves), every fourth tile group's scales
   const auto slot = [](int row, int c) { return BITS == kMx8 ? c ^ (row >> 1 & 7) : c ^ (row >> 2 & 3); };   // of piece c; and the piece of slot c
-  const uint8_t* const x0 = a.x + static_cast<int64_t>(m0) * a.ldx;
   uint32_t x_off[XD];
 #pragma unroll
   for (int p = 0; p < XD; ++p) {
     const int row = kRowsALoad * (XD * wave + p) + lane / kPieces;
-    x_off[p] = static_cast<uint32_t>(min(row, a.M - 1 - m0)) * static_cast<uint32_t>(a.ldx) + slot(row, lane % kPieces) * 16;
+    x_off[p] = static_cast<uint32_t>(min(row, a.M - 1)) * static_cast<uint32_t>(a.ldx) + slot(row, lane % kPieces) * 16;
   }
-  const uint8_t* w0[WD];
+  uint32_t w_off[WD];      // (with the lane's place in it)
   int w_to[WD];
 #pragma unroll
   for (int q = 0; q < WD; ++q) {      // a load too many is the last one again
     const int piece = min(WD * wave + q, kTiles - 1);
-    w0[q] = a.w + static_cast<int64_t>(min(tile0 + piece, a.n_tiles - 1)) * 1024;
+    w_off[q] = static_cast<uint32_t>(min(piece, a.n_tiles - 1)) * 1024u + lane * 16;
     w_to[q] = kXBytes + piece * 1024;
   }
   // a round's scales are kilobytes too: 64 rows of X or four tiles of W; which is which is a matter of addresses, as a branch in the loop
   // would part it into pieces between which the compiler moves products; a load too many is the last one again
   constexpr int kXItems = kXScales / 1024, kItems = kXItems + kTiles / 4, SD = (kItems + kWaves - 1) / kWaves;
-  const uint8_t* s0[SD];
   uint32_t s_off[SD];
-  int s_step[SD], s_to[SD];
+  int s_to[SD], s_step[SD];
 #pragma unroll
   for (int q = 0; q < SD; ++q) {
     const int item = min(SD * wave + q, kItems - 1);
     const bool of_x = item < kXItems;
-    s0[q] = of_x ? a.xs + static_cast<int64_t>(m0) * a.ldxs : reinterpret_cast<const uint8_t*>(a.ws);
-    s_off[q] = of_x ? static_cast<uint32_t>(min(64 * item + lane, a.M - 1 - m0)) * static_cast<uint32_t>(a.ldxs)
-                    : static_cast<uint32_t>(min(tile0 + 4 * (item - kXItems) + (lane >> 4), a.n_tiles - 1)) * 256u + (lane & 15) * 16;
     s_step[q] = of_x ? 16 : a.pitch * 256;
+    s_off[q] = of_x ? static_cast<uint32_t>(min(64 * item + lane, a.M - 1)) * static_cast<uint32_t>(a.ldxs)
+                    : static_cast<uint32_t>(min(4 * (item - kXItems) + (lane >> 4), a.n_tiles - 1)) * 256u + (lane & 15) * 16;
     s_to[q] = item * 1024;
   }
-  // step s of this part; past its end the last step again, so that every step has as many loads
-  auto fetch_scales = [&](int s) {
-    const int round = r_begin + min(s, n_steps - 1) / 4;
-#pragma unroll
-    for (int q = 0; q < SD; ++q) load_to_lds_16(s0[q] + static_cast<int64_t>(round) * s_step[q], s_off[q], lds_scales + (s / 4 & 1) * kScales + s_to[q]);
+  struct Tile {
+    int m0, tile0;                          // first row, first 16 columns
+    const uint8_t *x, *w, *scales[SD];      // of the part's first step
   };
-  auto fetch = [&](int s, unsigned char* to, int i) {     // load i of the batch
-    const int64_t abs = 4 * r_begin + min(s, n_steps - 1);
+  const auto tile_of = [&](int id) {
+    const int group = id / (8 * a.n_blocks), first = group * 8, rows_here = min(8, a.m_blocks - first), in = id - group * 8 * a.n_blocks;
+    Tile of;
+    of.m0 = min((first + in % rows_here) * kRows, max(a.M - kRows, 0));
+    of.tile0 = min(in / rows_here * kTiles, max(a.n_tiles - kTiles, 0));
+    of.x = a.x + static_cast<int64_t>(of.m0) * a.ldx + static_cast<int64_t>(r_begin) * (4 * kRowBytes);
+    of.w = a.w + (static_cast<int64_t>(r_begin) * 4 * a.pitch + of.tile0) * 1024;
+#pragma unroll
+    for (int q = 0; q < SD; ++q)
+      of.scales[q] = SD * wave + q < kXItems ? a.xs + static_cast<int64_t>(of.m0) * a.ldxs + static_cast<int64_t>(r_begin) * 16
+                                             : reinterpret_cast<const uint8_t*>(a.ws) + (static_cast<int64_t>(r_begin) * a.pitch + of.tile0) * 256;
+    return of;
+  };
+  Tile here = tile_of(id), ahead = here;      // of the results; of the batches that are sent past the tile's end
+  int turn = 0;               // rounds of the tiles before: a round's scales lie by the parity of its number
+  auto fetch_scales = [&](const Tile& of, int round, int at) {
+#pragma unroll
+    for (int q = 0; q < SD; ++q) load_to_lds_16(of.scales[q] + static_cast<int64_t>(round) * s_step[q], s_off[q], lds_scales + (at & 1) * kScales + s_to[q]);
+  };
+  auto fetch = [&](const Tile& of, int s, unsigned char* to, int i) {     // load i of step s's batch
     if (i < XD)
-      load_to_lds_16(x0 + abs * kRowBytes, x_off[i], to + (XD * wave + i) * 1024);
+      load_to_lds_16(of.x + static_cast<int64_t>(s) * kRowBytes, x_off[i], to + (XD * wave + i) * 1024);
     else
-      load_to_lds_16(w0[i - XD] + abs * (static_cast<int64_t>(a.pitch) * 1024), lane * 16, to + w_to[i - XD]);
+      load_to_lds_16(of.w + static_cast<int64_t>(s) * (static_cast<int64_t>(a.pitch) * 1024), w_off[i - XD], to + w_to[i - XD]);
   };
 
   mx_f32x16 acc[MT][TN];
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int tn = 0; tn < TN; ++tn)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[t][tn][r] = 0.f;
 
   // this lane's places in a stage: a piece of X row 32 (MT wr + t) + j is at x_at with bits exchanged; W
   const int x_at = (wr * 32 * MT + j) * kRowBytes + slot(j, h) * 16;
@@ -285,8 +300,8 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
     u32x4 x[MT];           // of a round: a row's sixteen bytes; in use turned so that this lane's blocks are bytes 0 and 2 of the step's word
     uint32_t w[TN][2];
   };
-  auto read_scales = [&](int round, Scales& to) {
-    const unsigned char* sc = lds_scales + (round & 1) * kScales;
+  auto read_scales = [&](int at, Scales& to) {
+    const unsigned char* sc = lds_scales + (at & 1) * kScales;
 #pragma unroll
     for (int t = 0; t < MT; ++t) to.x[t] = *reinterpret_cast<const u32x4*>(sc + (wr * 32 * MT + 32 * t + j) * 16);
 #pragma unroll
@@ -308,9 +323,9 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
 
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
-    if (s % 4 == 0) fetch_scales(s);
+    if (s % 4 == 0) fetch_scales(here, min(s, n_steps - 1) / 4, s / 4);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) fetch(s, lds + s * kStage, i);
+    for (int i = 0; i < kBatch; ++i) fetch(here, min(s, n_steps - 1), lds + s * kStage, i);
   }
   batch_landed();
   __syncthreads();
@@ -323,142 +338,199 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
 #pragma unroll
   for (int tn = 0; tn < TN; ++tn) wo[0][tn] = read_w(lds, 0, tn);
   unsigned char *now = lds, *last = lds + (STAGES - 1) * kStage;     // the stage of this step; where the batch goes
-  for (int r = 0; r < n_rounds; ++r) {
-    auto step = [&](auto uc) {
-      constexpr int u = decltype(uc)::value;
-      const int s = 4 * r + u;
-      unsigned char* next = now == lds + (STAGES - 1) * kStage ? lds : now + kStage;
-      if constexpr (u == (9 - STAGES) % 4) fetch_scales(s + STAGES - 1);
+  for (;;) {
+    if constexpr (kStays) {
+      place += gridDim.x;
+      id = tile_at(place);
+      if (id < total) {
+        ahead = tile_of(id);
+      } else {      // this tile's last round again, which the caches hold
+        ahead = here;
+        ahead.x += static_cast<int64_t>(n_rounds - 1) * (4 * kRowBytes);
+        ahead.w += static_cast<int64_t>(n_rounds - 1) * 4 * a.pitch * 1024;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const int kk = g / MT, t = g % MT;
-        if (g == kGroups - kAhead) {
-          batch_landed();
-          __syncthreads();
-          if constexpr (u == 3) read_scales(r + 1, scales_next);
-        }
-        const unsigned char* from = g >= kGroups - kAhead ? next : now;
-        const int gn = (g + kAhead) % kGroups;
-        const int xscale = static_cast<int>(scales.x[t][u]);
-        const mx_i32x8 x = xo[g % kRing].whole();
-#pragma unroll
-        for (int tn = 0; tn < TN; ++tn) {
-          // in front of every product a piece of the operands of the group behind, and a load of the batch here and there
-          constexpr int kParts = BITS == kMx8 ? 2 : 1;
-#pragma unroll
-          for (int part = 0; part < kParts; ++part)
-            if (TN == 1 || tn == part) xo[(g + kAhead) % kRing].part[part] = read_x(from, gn / MT, gn % MT, part);
-          if (gn % MT == 0) wo[gn / MT][tn] = read_w(from, gn / MT, tn);
-          constexpr int kSlots = (kGroups - kAhead) * TN;
-          const int slot_at = g * TN + tn;
-          if (slot_at < kSlots) {
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-              if (i * kSlots / kBatch == slot_at) fetch(s + STAGES - 1, last, i);
-          }
-          // the byte of W's scale word is the step inside the round, that of X's the half
-          if (kk == 0)
-            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[0][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(scales.w[tn][0]), 0,
-                                                                         xscale);
-          else
-            acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[1][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(scales.w[tn][1]), 2,
-                                                                         xscale);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int q = 0; q < SD; ++q) ahead.scales[q] += static_cast<int64_t>(n_rounds - 1) * s_step[q];
       }
-      if constexpr (u == 3) use_scales(scales_next);
-      last = now;
-      now = next;
-    };
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
-    step(std::integral_constant<int, 2>{});
-    step(std::integral_constant<int, 3>{});
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the batches past the end: nothing may land in what follows
-  __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t][tn][r] = 0.f;
+    for (int r = 0; r < n_rounds; ++r) {
+      auto step = [&](auto uc) {
+        constexpr int u = decltype(uc)::value;
+        const int s = 4 * r + u;
+        unsigned char* next = now == lds + (STAGES - 1) * kStage ? lds : now + kStage;
+        // the step whose batch is sent: STAGES - 1 further, which may be one of the next tile (without one: of this tile again)
+        const bool over = s + STAGES - 1 >= n_steps;
+        const int f = kStays ? s + STAGES - 1 - (over ? n_steps : 0) : min(s + STAGES - 1, n_steps - 1);
+        Tile of = here;
+        if constexpr (kStays) {
+          of.x = over ? ahead.x : here.x;
+          of.w = over ? ahead.w : here.w;
+#pragma unroll
+          for (int q = 0; q < SD; ++q) of.scales[q] = over ? ahead.scales[q] : here.scales[q];
+        }
+        if constexpr (u == (9 - STAGES) % 4) fetch_scales(of, f / 4, turn + (s + STAGES - 1) / 4);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const int kk = g / MT, t = g % MT;
+          if (g == kGroups - kAhead) {
+            batch_landed();
+            __syncthreads();
+            if constexpr (u == 3) read_scales(turn + r + 1, scales_next);
+          }
+          const unsigned char* from = g >= kGroups - kAhead ? next : now;
+          const int gn = (g + kAhead) % kGroups;
+          const int xscale = static_cast<int>(scales.x[t][u]);
+          const mx_i32x8 x = xo[g % kRing].whole();
+#pragma unroll
+          for (int tn = 0; tn < TN; ++tn) {
+            // in front of every product a piece of the operands of the group behind, and a load of the batch here and there
+            constexpr int kParts = BITS == kMx8 ? 2 : 1;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+              if (TN == 1 || tn == part) xo[(g + kAhead) % kRing].part[part] = read_x(from, gn / MT, gn % MT, part);
+            if (gn % MT == 0) wo[gn / MT][tn] = read_w(from, gn / MT, tn);
+            constexpr int kSlots = (kGroups - kAhead) * TN;
+            const int slot_at = g * TN + tn;
+            if (slot_at < kSlots) {
+#pragma unroll
+              for (int i = 0; i < kBatch; ++i)
+                if (i * kSlots / kBatch == slot_at) fetch(of, f, last, i);
+            }
+            // the byte of W's scale word is the step inside the round, that of X's the half
+            if (kk == 0)
+              acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[0][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(scales.w[tn][0]), 0,
+                                                                           xscale);
+            else
+              acc[t][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand4(wo[1][tn]), x, acc[t][tn], 4, kFormat, u, static_cast<int>(scales.w[tn][1]), 2,
+                                                                           xscale);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        if constexpr (u == 3) use_scales(scales_next);
+        last = now;
+        now = next;
+      };
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
+      step(std::integral_constant<int, 2>{});
+      step(std::integral_constant<int, 3>{});
+    }
+    // the batches past the end of the last tile: nothing may land in what is another workgroup's then (in front of the results, which nothing waits for)
+    if (!kStays || id >= total) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int m_here = here.m0, n_here = here.tile0 * 16 + wc * (32 * TN);
 
-  // acc[t][tn][r] = C[m0 + 32 (MT wr + t) + j][n0 + 32 tn + 8 (r / 4) + 4 h + r % 4].  Stored as they are, a lane's four columns are scraps of 4
-  // to 16 bytes of a row; they go through a part of LDS that belongs to the wave and leave as whole runs of a row, 16 bytes a lane.
-  constexpr int kRun = kGate ? (EPI == kMxGate8 ? 16 * TN : 8 * TN) : (EPI == kMxBf16 ? 64 * TN : 128);   // bytes of a row
-  constexpr int kPitch = kRun + 16, kLanes = kRun / 16, kRowsAPass = kWave / kLanes;
-  static_assert(kWaves * 32 * kPitch <= STAGES * kStage, "the wave's part of the stages");
-  unsigned char* const mine = lds + wave * (32 * kPitch);
-  auto settle = [] {     // what the wave's lanes wrote is there for its other lanes
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  };
-  auto leave = [&](int row0, unsigned char* out, int64_t pitch) {     // out: the run's place in row row0
-    settle();
+    // acc[t][tn][r] = C[m_here + 32 (MT wr + t) + j][n_here + 32 tn + 8 (r / 4) + 4 h + r % 4].  Stored as they are, a lane's four columns are scraps of 4
+    // to 16 bytes of a row; they go through a part of LDS that belongs to the wave and leave as whole runs of a row, 16 bytes a lane.
+    constexpr int kRun = kGate ? (EPI == kMxGate8 ? 16 * TN : 8 * TN) : (EPI == kMxBf16 ? 64 * TN : 128);   // bytes of a row
+    constexpr int kPitch = kRun + 16, kLanes = kRun / 16, kRowsAPass = kWave / kLanes;
+    // The one stage that is free is that of the last step, `last`; the others hold, or wait for, batches of the steps behind.  So 16 rows at a time.
+    static_assert(kWaves * 16 * kPitch <= kStage, "the wave's part of the stage");
+    unsigned char* const mine = last + wave * (16 * kPitch);
+    auto settle = [] {     // what the wave's lanes wrote is there for its other lanes
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    auto leave = [&](int row0, unsigned char* out, int64_t pitch, auto&& put) {     // out: the run's place in row row0; put: writes this lane's part of a row
 #pragma unroll
-    for (int i = 0; i < (32 + kRowsAPass - 1) / kRowsAPass; ++i) {
-      const int rr = kRowsAPass * i + lane / kLanes, piece = lane % kLanes;
-      if (rr < 32 && row0 + rr < a.M)
-        *reinterpret_cast<u32x4*>(out + rr * pitch + piece * 16) = *reinterpret_cast<const u32x4*>(mine + rr * kPitch + piece * 16);
-    }
-    settle();
-  };
-  if constexpr (kGate) {
-    constexpr int kBits = EPI == kMxGate8 ? kMx8 : kMx4;
-    if (n0 / 16 >= a.n_tiles) return;             // whole blocks: the columns are a multiple of 512
+      for (int half = 0; half < 2; ++half) {
+        if (j >> 4 == half) put(mine + (j & 15) * kPitch);
+        settle();
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int row0 = m0 + 32 * (MT * wr + t);
-#pragma unroll
-      for (int b = 0; b < TN / 2; ++b) {          // blocks of 32 results
-        float4 v[2][2];
-        uint32_t most = 0;
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const mx_f32x16& c = acc[t][2 * b + p];
-            v[p][q] = float4{mx_silu_mul(c[4 * q], c[4 * q + 8]), mx_silu_mul(c[4 * q + 1], c[4 * q + 9]), mx_silu_mul(c[4 * q + 2], c[4 * q + 10]),
-                             mx_silu_mul(c[4 * q + 3], c[4 * q + 11])};
-            most = max(most, mx_max4(v[p][q]));
-          }
-        const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
-        const uint32_t code = mx_code<kBits>(max(both[0], both[1]));
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int q = 0; q < 2; ++q) mx_store4<kBits>(mine + j * kPitch, 32 * b + 16 * p + 8 * q + 4 * h, mx_pack4<kBits>(v[p][q], code));
-        if (h == 0 && row0 + j < a.M) a.out_scales[static_cast<int64_t>(row0 + j) * a.ldos + n0 / 64 + b] = static_cast<uint8_t>(code);
+        for (int i = 0; i < (16 + kRowsAPass - 1) / kRowsAPass; ++i) {
+          const int rr = kRowsAPass * i + lane / kLanes, piece = lane % kLanes;
+          if (rr < 16 && row0 + 16 * half + rr < a.M)
+            *reinterpret_cast<u32x4*>(out + (16 * half + rr) * pitch + piece * 16) = *reinterpret_cast<const u32x4*>(mine + rr * kPitch + piece * 16);
+        }
+        settle();
       }
-      leave(row0, static_cast<uint8_t*>(a.out) + static_cast<int64_t>(row0) * a.ldo + n0 / 2 * kBits / 8, a.ldo);
-    }
-  } else {
-    const bool whole = (a.ldo & 7) == 0 && n0 + 32 * TN <= a.N;      // the same in all lanes
+    };
+    if constexpr (kGate) {
+      constexpr int kBits = EPI == kMxGate8 ? kMx8 : kMx4;
+      // (whole blocks: the columns are a multiple of 512)
+      const int row_tiles = n_here / 16 < a.n_tiles ? MT : 0;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int row0 = m0 + 32 * (MT * wr + t);
-      if (!whole) {
+      for (int t = 0; t < MT; ++t) {
+        if (t >= row_tiles) break;
+        const int row0 = m_here + 32 * (MT * wr + t);
+        uint32_t packed[TN / 2][2][2];
 #pragma unroll
-        for (int tn = 0; tn < TN; ++tn)
+        for (int b = 0; b < TN / 2; ++b) {          // blocks of 32 results
+          float4 v[2][2];
+          uint32_t most = 0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            mx_store_sums<EPI>(a, blockIdx.y, row0 + j, n0 + 32 * tn + 8 * q + 4 * h,
-                               mx_f32x4{acc[t][tn][4 * q], acc[t][tn][4 * q + 1], acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3]});
-      } else if constexpr (EPI == kMxBf16) {
+          for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int tn = 0; tn < TN; ++tn)
+            for (int q = 0; q < 2; ++q) {
+              const mx_f32x16& c = acc[t][2 * b + p];
+              v[p][q] = float4{mx_silu_mul(c[4 * q], c[4 * q + 8]), mx_silu_mul(c[4 * q + 1], c[4 * q + 9]), mx_silu_mul(c[4 * q + 2], c[4 * q + 10]),
+                               mx_silu_mul(c[4 * q + 3], c[4 * q + 11])};
+              most = max(most, mx_max4(v[p][q]));
+            }
+          const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+          const uint32_t code = mx_code<kBits>(max(both[0], both[1]));
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint2*>(mine + j * kPitch + (32 * tn + 8 * q + 4 * h) * 2) =
-                uint2{pack_bf16x2(acc[t][tn][4 * q], acc[t][tn][4 * q + 1]), pack_bf16x2(acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3])};
-        leave(row0, reinterpret_cast<unsigned char*>(static_cast<bf16*>(a.out) + static_cast<int64_t>(row0) * a.ldo + n0), static_cast<int64_t>(a.ldo) * 2);
-      } else {
+          for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int tn = 0; tn < TN; ++tn) {
+            for (int q = 0; q < 2; ++q) packed[b][p][q] = mx_pack4<kBits>(v[p][q], code);
+          if (h == 0 && row0 + j < a.M) a.out_scales[static_cast<int64_t>(row0 + j) * a.ldos + n_here / 64 + b] = static_cast<uint8_t>(code);
+        }
+        leave(row0, static_cast<uint8_t*>(a.out) + static_cast<int64_t>(row0) * a.ldo + n_here / 2 * kBits / 8, a.ldo, [&](uint8_t* row) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<mx_f32x4*>(mine + j * kPitch + (8 * q + 4 * h) * 4) =
-                mx_f32x4{acc[t][tn][4 * q], acc[t][tn][4 * q + 1], acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3]};
-          leave(row0, reinterpret_cast<unsigned char*>(static_cast<float*>(a.out) + (static_cast<int64_t>(blockIdx.y) * a.M + row0) * a.ldo + n0 + 32 * tn), static_cast<int64_t>(a.ldo) * 4);
+          for (int b = 0; b < TN / 2; ++b)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) mx_store4<kBits>(row, 32 * b + 16 * p + 8 * q + 4 * h, packed[b][p][q]);
+        });
+      }
+    } else {
+      const bool whole = (a.ldo & 7) == 0 && n_here + 32 * TN <= a.N;      // the same in all lanes
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const int row0 = m_here + 32 * (MT * wr + t);
+        if (!whole) {
+#pragma unroll
+          for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              mx_store_sums<EPI>(a, blockIdx.y, row0 + j, n_here + 32 * tn + 8 * q + 4 * h,
+                                 mx_f32x4{acc[t][tn][4 * q], acc[t][tn][4 * q + 1], acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3]});
+        } else if constexpr (EPI == kMxBf16) {
+          leave(row0, reinterpret_cast<unsigned char*>(static_cast<bf16*>(a.out) + static_cast<int64_t>(row0) * a.ldo + n_here), static_cast<int64_t>(a.ldo) * 2,
+                [&](unsigned char* row) {
+#pragma unroll
+                  for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                      *reinterpret_cast<uint2*>(row + (32 * tn + 8 * q + 4 * h) * 2) =
+                          uint2{pack_bf16x2(acc[t][tn][4 * q], acc[t][tn][4 * q + 1]), pack_bf16x2(acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3])};
+                });
+        } else {
+#pragma unroll
+          for (int tn = 0; tn < TN; ++tn)
+            leave(row0,
+                  reinterpret_cast<unsigned char*>(static_cast<float*>(a.out) + (static_cast<int64_t>(blockIdx.y) * a.M + row0) * a.ldo + n_here + 32 * tn),
+                  static_cast<int64_t>(a.ldo) * 4,
+                  [&](unsigned char* row) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                      *reinterpret_cast<mx_f32x4*>(row + (8 * q + 4 * h) * 4) =
+                          mx_f32x4{acc[t][tn][4 * q], acc[t][tn][4 * q + 1], acc[t][tn][4 * q + 2], acc[t][tn][4 * q + 3]};
+                  });
         }
       }
     }
+    if constexpr (!kStays) break;
+    if (id >= total) break;
+    here = ahead;
+    turn += n_rounds;
+    __syncthreads();       // all results are out of the stage
   }
 }
 
@@ -480,8 +552,10 @@ int mx_tiles_launch(MxArgs a, int splits, hipStream_t s) {
   if (const int e = ask_lds(asked, kLds, {reinterpret_cast<const void*>(kernel)})) return e;
   a.m_blocks = (a.M + kRows - 1) / kRows;
   a.n_blocks = (a.n_tiles + kTiles - 1) / kTiles;
-  const int per_xcd = (a.m_blocks * a.n_blocks + 7) / 8;
-  kernel<<<dim3(8 * per_xcd, splits), RW * CW * kWave, kLds, s>>>(a);
+  // workgroups that stay: as many as run at once, each going on to its next tile while the results of the one before leave
+  const int places = (a.m_blocks * a.n_blocks + 7) / 8 * 8;
+  constexpr int kByLds = 160 * 1024 / kLds, kByWaves = 4 * WAVES_A_SIMD / (RW * CW), kHeld = kByLds < kByWaves ? kByLds : kByWaves, kUnits = 256;
+  kernel<<<dim3(STAGES <= 5 && splits == 1 ? min(places, kHeld * kUnits) : places, splits), RW * CW * kWave, kLds, s>>>(a);
   return launch_status();
 }
 

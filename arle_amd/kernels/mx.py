@@ -316,25 +316,28 @@ def lay_weight(rows: MXRows, gated: bool = False) -> MXWeight:
 
 _EPI_F32, _EPI_GATE = F32, {"mxfp8": 2, "mxfp4": 3}                         # (sums leave as the type whose code this is)
 ROW_VARIANTS = (0, 1)                                                       # of up to 16 rows (mx_gemm_rows_kernel)
-# variant of mx_gemm_tiles_kernel -> rows, columns, workgroups a compute unit holds, us to start and end a workgroup, and us of 128 k for one workgroup
+# variant of mx_gemm_tiles_kernel -> rows, columns, workgroups a compute unit holds, us to start and end a launch, and us of 128 k for one workgroup
 # alone and for a compute unit that is as full as all others, for rows of 8 bits and of 4.  What they were read from (MI355X, us in a captured graph,
 # 2.4 of which are the launch; rows x N x K, 8 bits if not said):
 #                                  32x64  64x128  128x128  128x256  256x256  128x192  256x192
 #   64 x 2,560 x 9,728              16.3    26.4     36.1     41.5     75.5     35.5     58.8
 #   128 x 6,144 x 2,560             10.2    10.4     14.3     17.6     24.8     17.2     20.8
 #   512 x 2,560 x 9,728             36.8    25.3     39.0     48.3     80.8     43.3     67.4
-#   2,048 x 2,560 x 9,728                   64.9     54.6     48.3     77.6     43.2     64.6
-#   2,048 x 6,144 x 2,560                   34.8     29.5     33.3     30.8     32.8     28.1
-#   4,096 x 6,144 x 4,096                            88.2     82.7     88.5     90.2     78.8
-#   4,096 x 4,096 x 12,288                          166.4    144.4    133.2    167.8    184.6
-#   2,048 x 2,560 x 9,728, 4 bits                    40.4     34.4     52.6     34.3     46.7
-#   4,096 x 6,144 x 4,096, 4 bits                    73.0     63.6     61.9     71.8     58.6
+#   2,048 x 2,560 x 9,728                   64.9     52.3     44.3     77.6     44.1     63.5
+#   2,048 x 6,144 x 2,560                   34.8     28.1     31.0     30.4     30.5     27.1
+#   4,096 x 6,144 x 4,096                            85.3     77.6     86.6     85.3     75.3
+#   4,096 x 4,096 x 12,288                          158.8    143.6    134.0    164.4    181.7
+#   8,192 x 6,144 x 2,560                           103.3     98.6     93.3    110.7     94.9
+#   8,192 x 2,560 x 9,728                           156.6    154.1    180.0    171.7    152.2
+#   2,048 x 2,560 x 9,728, 4 bits                    38.3     33.0     50.6     34.0     46.5
+#   4,096 x 6,144 x 4,096, 4 bits                    67.1     59.2     60.2     69.6     55.2
 #   gate|up, 64 x 9,728 x 2,560             12.3     14.1     16.4     26.6
-#   gate|up, 2,048 x 9,728 x 2,560         143.0     84.1     86.1     91.9
-#   gate|up, 4,096 x 12,288 x 4,096        546.3    333.2    310.8    282.9
-_TILES = {2: (32, 64, 2, 1.5, 0.15, 0.36, 0.15, 0.36), 3: (64, 128, 1, 2.5, 0.28, 0.28, 0.25, 0.25), 4: (128, 128, 2, 2.5, 0.43, 0.80, 0.38, 0.66),
-          5: (128, 256, 1, 3.0, 0.55, 0.74, 0.30, 0.52), 6: (256, 256, 1, 5.0, 0.95, 1.30, 0.55, 0.77), 7: (128, 192, 1, 3.0, 0.48, 0.56, 0.36, 0.45),
-          8: (256, 192, 1, 4.0, 0.80, 1.07, 0.53, 0.75)}
+#   gate|up, 2,048 x 9,728 x 2,560         143.0     81.4     78.9     85.3
+#   gate|up, 4,096 x 12,288 x 4,096        546.3    325.0    298.1    276.2
+#   the same, 4 bits                                279.4    241.4    197.2
+_TILES = {2: (32, 64, 2, 1.5, 0.15, 0.36, 0.15, 0.36), 3: (64, 128, 1, 2.5, 0.28, 0.28, 0.25, 0.25), 4: (128, 128, 2, 2.5, 0.43, 0.78, 0.38, 0.68),
+          5: (128, 256, 1, 3.0, 0.48, 0.715, 0.30, 0.55), 6: (256, 256, 1, 5.0, 0.95, 1.32, 0.55, 0.92), 7: (128, 192, 1, 3.0, 0.44, 0.59, 0.36, 0.47),
+          8: (256, 192, 1, 4.0, 0.80, 1.05, 0.53, 0.73)}
 _PLAIN_TILES = (2, 7, 8)  # whose waves own no whole blocks of 32 gated results
 _UNITS = 256             # compute units
 _SUM_US, _STACK_BYTES_A_US = 5.0, 5e6      # a launch more, which an eager caller pays the host for too; the stack written and read
@@ -344,11 +347,11 @@ def _tiles_us(variant: int, M: int, N: int, k_tiles: int, bits: int, splits: int
     """What a product is expected to take, as far as variants and parts of K are compared by it."""
     rows, cols, held, start, *us = _TILES[variant]
     alone, full = us[:2] if bits == 8 else us[2:]
-    groups = -(-M // rows) * -(-N // cols) * splits
-    share = groups / (_UNITS * held)
-    turns = max(1.0, share) if held > 1 else -(-groups // _UNITS)      # a unit that holds several starts the next one while others run
-    busy = 0.0 if held > 1 and groups <= _UNITS else min(1.0, share)   # and up to one workgroup a unit each has its unit to itself
-    return turns * (4 * -(-k_tiles // (4 * splits)) * (alone + (full - alone) * busy) + start)
+    turns, rest = divmod(-(-M // rows) * -(-N // cols) * splits, _UNITS * held)
+    # the last turn has fewer workgroups; up to one a unit each of them has its unit to itself
+    busy = 0.0 if held > 1 and rest <= _UNITS else rest / (_UNITS * held)
+    steps = 4 * -(-k_tiles // (4 * splits))
+    return start / 2 + turns * (steps * full + start / 2) + (steps * (alone + (full - alone) * busy) + start / 2 if rest else 0.0)
 
 
 @functools.lru_cache(maxsize=4096)

@@ -186,3 +186,25 @@ def test_tuning_leaves_such_projections_alone(tmp_path):
     engine.tune_products(rows=[1, 8])
     engine.add_request("x")
     assert torch.isfinite(engine.step([StepEntry("x", [1, 2, 3], [2])])).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("K", [130, 1100, 1600])
+def test_workgroups_with_several_tiles(form, K):
+    """Products of more tiles than workgroups that run at once, whose last row and column blocks overlap the ones in front, with one, three and
+    four rounds of K: exact, as numbers up to 3 and weights up to 6 with scales from 1/4 to 4 have sums under 2^20 of multiples of 1/32."""
+    M, N = 4100, 4700
+    few = torch.tensor([0, 2, 4, 5, 8, 10, 12, 13] if form == "mxfp4" else [0, 0x38, 0x40, 0x44, 0x80, 0xB8, 0xC0, 0xC4], dtype=torch.uint8)
+    xe, we = few[torch.randint(0, 8, (M, K), generator=_g(1))], torch.randint(0, 16, (N, K), generator=_g(2), dtype=torch.uint8)
+    xs, ws = (torch.randint(125, 130, (n, -(-K // 32)), generator=_g(n), dtype=torch.uint8) for n in (M, N))
+    x, wide = mx.rows_from_codes(xe.to(DEV), xs.to(DEV), K, form), mx.rows_from_codes(we.to(DEV), ws.to(DEV), K, "mxfp4")
+    w, gated = mx.lay_weight(wide), mx.lay_weight(wide, gated=True)
+    want = (plain.dequantize(xe, xs, form).float().to(DEV).double() @ plain.dequantize(we, ws, "mxfp4").float().to(DEV).double().T)
+    gate = plain.unpack(mx.gate_up_act(x, gated, form, variant=3))      # whose workgroups have one tile each
+    for variant in sorted(mx._TILES):
+        for dtype in (torch.float32, torch.bfloat16):
+            assert torch.equal(mx.gemm(x, w, dtype, variant=variant), want.to(dtype)), (variant, dtype)
+        if variant not in mx._PLAIN_TILES:
+            assert all(torch.equal(p, q) for p, q in zip(gate, plain.unpack(mx.gate_up_act(x, gated, form, variant=variant)))), variant
+    parts = mx.gemm(x, w, torch.float32, partials_ok=True, variant=5, splits=min(2, x.padded // 512))
+    assert torch.equal(parts.double().sum(0) if parts.dim() == 3 else parts.double(), want)
