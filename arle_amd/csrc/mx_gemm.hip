@@ -220,18 +220,20 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
 
   // what the wave fetches: XD kilobytes of rows of X, tiles WD wave .. of W, 64 rows' scales (the first waves), every fourth tile group's scales
   const auto slot = [](int row, int c) { return BITS == kMx8 ? c ^ (row >> 1 & 7) : c ^ (row >> 2 & 3); };   // of piece c; and the piece of slot c
+  // a tile's rows and 16 columns that there are: nothing past them may be read (64 rows' scales are fetched for a tile of 32 too)
+  const int last_row = min(a.M, kRows) - 1, last_tile = min(a.n_tiles, kTiles) - 1;
   uint32_t x_off[XD];
 #pragma unroll
   for (int p = 0; p < XD; ++p) {
     const int row = kRowsALoad * (XD * wave + p) + lane / kPieces;
-    x_off[p] = static_cast<uint32_t>(min(row, a.M - 1)) * static_cast<uint32_t>(a.ldx) + slot(row, lane % kPieces) * 16;
+    x_off[p] = static_cast<uint32_t>(min(row, last_row)) * static_cast<uint32_t>(a.ldx) + slot(row, lane % kPieces) * 16;
   }
   uint32_t w_off[WD];      // (with the lane's place in it)
   int w_to[WD];
 #pragma unroll
   for (int q = 0; q < WD; ++q) {      // a load too many is the last one again
     const int piece = min(WD * wave + q, kTiles - 1);
-    w_off[q] = static_cast<uint32_t>(min(piece, a.n_tiles - 1)) * 1024u + lane * 16;
+    w_off[q] = static_cast<uint32_t>(min(piece, last_tile)) * 1024u + lane * 16;
     w_to[q] = kXBytes + piece * 1024;
   }
   // a round's scales are kilobytes too: 64 rows of X or four tiles of W; which is which is a matter of addresses, as a branch in the loop
@@ -244,8 +246,8 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
     const int item = min(SD * wave + q, kItems - 1);
     const bool of_x = item < kXItems;
     s_step[q] = of_x ? 16 : a.pitch * 256;
-    s_off[q] = of_x ? static_cast<uint32_t>(min(64 * item + lane, a.M - 1)) * static_cast<uint32_t>(a.ldxs)
-                    : static_cast<uint32_t>(min(4 * (item - kXItems) + (lane >> 4), a.n_tiles - 1)) * 256u + (lane & 15) * 16;
+    s_off[q] = of_x ? static_cast<uint32_t>(min(64 * item + lane, last_row)) * static_cast<uint32_t>(a.ldxs)
+                    : static_cast<uint32_t>(min(4 * (item - kXItems) + (lane >> 4), last_tile)) * 256u + (lane & 15) * 16;
     s_to[q] = item * 1024;
   }
   struct Tile {

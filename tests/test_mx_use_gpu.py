@@ -208,3 +208,45 @@ def test_workgroups_with_several_tiles(form, K):
             assert all(torch.equal(p, q) for p, q in zip(gate, plain.unpack(mx.gate_up_act(x, gated, form, variant=variant)))), variant
     parts = mx.gemm(x, w, torch.float32, partials_ok=True, variant=5, splits=min(2, x.padded // 512))
     assert torch.equal(parts.double().sum(0) if parts.dim() == 3 else parts.double(), want)
+
+
+def _at_the_end(t):
+    """The same numbers in the last bytes of an allocation that ends with its mapping (of its own, a multiple of 2 MiB): a kernel that reads past
+    what it was given, wherever that is the last of it, does not get away with it."""
+    whole = torch.empty(32 * 2**20, dtype=torch.uint8, device=DEV)
+    flat = t.contiguous().view(torch.uint8).flatten()
+    whole[-flat.numel():] = flat
+    return whole[-flat.numel():].view(t.dtype).view(t.shape)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_operands_at_the_end_of_their_memory(form):
+    """Every variant with rows and columns that fill its last tile, end inside it, or are fewer than it has."""
+    torch.cuda.empty_cache()
+    N, K = 600, 1100
+    q = mx.quantize(torch.randn(520, K, generator=_g(1)).to(DEV), form)
+    held = mx.quantize(torch.randn(N, K, generator=_g(2)).to(DEV), "mxfp4")
+    w, wg = mx.lay_weight(held), mx.lay_weight(held, gated=True)
+    ends = [mx.MXWeight(_at_the_end(v.tiles), _at_the_end(v.scales), v.n, v.k, v.gated) for v in (w, wg)]
+    for M in (1, 16, 17, 32, 33, 64, 65, 100, 130, 256, 300, 520):
+        rows = q.part(0, M)
+        x = mx.MXRows(_at_the_end(rows.elements), _at_the_end(rows.scales), K, form)
+        for variant in range(9):
+            if variant > 1 or M <= 16:
+                assert torch.equal(mx.gemm(x, ends[0], torch.float32, variant=variant), mx.gemm(rows, w, torch.float32, variant=variant)), (M, variant)
+        for variant in (3, 4, 5, 6):
+            got, want = mx.gate_up_act(x, ends[1], form, variant=variant), mx.gate_up_act(rows, wg, form, variant=variant)
+            assert all(torch.equal(a, b) for a, b in zip(plain.unpack(got), plain.unpack(want))), (M, variant)
+        assert torch.equal(mx.values(x), mx.values(rows))
+    for n in (1, 16, 100):      # fewer columns than a tile has
+        few = mx.lay_weight(mx.quantize(torch.randn(n, K, generator=_g(n)).to(DEV), "mxfp4"))
+        end = mx.MXWeight(_at_the_end(few.tiles), _at_the_end(few.scales), n, K)
+        for variant in range(2, 9):
+            assert torch.equal(mx.gemm(x, end, torch.float32, variant=variant), mx.gemm(rows, few, torch.float32, variant=variant)), (n, variant)
+    for T, W in ((1, 264), (5, 1530), (1100, 513)):
+        numbers = torch.randn(T, W, generator=_g(T)).bfloat16().to(DEV)
+        assert all(torch.equal(a, b) for a, b in zip(plain.unpack(mx.quantize(_at_the_end(numbers), form)), plain.unpack(mx.quantize(numbers, form))))
+        residual, weight = torch.randn(T, W, generator=_g(3)).to(DEV), _at_the_end(torch.ones(W, device=DEV))
+        a = mx.add_rmsnorm(_at_the_end(residual), _at_the_end(torch.stack([numbers, numbers])), weight, 1e-6, form)
+        b = mx.add_rmsnorm(residual, torch.stack([numbers, numbers]), weight, 1e-6, form)
+        assert all(torch.equal(p, q) for p, q in zip(plain.unpack(a), plain.unpack(b)))
