@@ -151,12 +151,32 @@ __global__ __launch_bounds__(WAVES* kWave) void mx_gemm_rows_kernel(const MxArgs
 #pragma unroll
   for (int c = 0; c < CT; ++c) parts[wave][c][g * kSub + i] = acc[c];
   __syncthreads();
-  for (int item = tid; item < 16 * CT * 4; item += WAVES * kWave) {      // (row, four columns)
-    const int r = item / (CT * 4), q = item % (CT * 4), at = (q & 3) * kSub + r;
-    mx_f32x4 sum = parts[0][q >> 2][at];
+  if constexpr (EPI == kMxGate8 || EPI == kMxGate4) {
+    static_assert(CT == 4, "a block of 32 results is two tiles of gate and two of up columns");
+    constexpr int kBits = EPI == kMxGate8 ? kMx8 : kMx4;
+    if (tid < 128) {                                                     // (row, four results): eight neighbouring lanes have a block
+      const int r = tid >> 3, q = tid & 7, at = (q & 3) * kSub + r;
+      mx_f32x4 gate = parts[0][q >> 2 << 1][at], up = parts[0][(q >> 2 << 1) + 1][at];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) sum += parts[w][q >> 2][at];
-    mx_store_sums<EPI>(a, blockIdx.y, r, 16 * ct0 + 4 * q, sum);
+      for (int w = 1; w < WAVES; ++w) {
+        gate += parts[w][q >> 2 << 1][at];
+        up += parts[w][(q >> 2 << 1) + 1][at];
+      }
+      const float4 v = {mx_silu_mul(gate[0], up[0]), mx_silu_mul(gate[1], up[1]), mx_silu_mul(gate[2], up[2]), mx_silu_mul(gate[3], up[3])};
+      const uint32_t code = mx_code<kBits>(mx_lanes_max<8>(mx_max4(v)));
+      if (r < a.M) {
+        mx_store4<kBits>(static_cast<uint8_t*>(a.out) + static_cast<int64_t>(r) * a.ldo, 8 * ct0 + 4 * q, mx_pack4<kBits>(v, code));
+        if (q == 0) a.out_scales[static_cast<int64_t>(r) * a.ldos + ct0 / 4] = static_cast<uint8_t>(code);
+      }
+    }
+  } else {
+    for (int item = tid; item < 16 * CT * 4; item += WAVES * kWave) {    // (row, four columns)
+      const int r = item / (CT * 4), q = item % (CT * 4), at = (q & 3) * kSub + r;
+      mx_f32x4 sum = parts[0][q >> 2][at];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) sum += parts[w][q >> 2][at];
+      mx_store_sums<EPI>(a, blockIdx.y, r, 16 * ct0 + 4 * q, sum);
+    }
   }
 }
 
@@ -574,6 +594,7 @@ int mx_launch(int variant, const MxArgs& a, int splits, hipStream_t s) {
     case 6: return mx_tiles_launch<BITS, EPI, 4, 2, 2, 4, BITS == kMx8 ? 3 : 4, 2>(a, splits, s);
     case 7: if constexpr (!kGate) return mx_tiles_launch<BITS, EPI, 2, 3, 2, 2, 5, 1>(a, splits, s); else break;
     case 8: if constexpr (!kGate) return mx_tiles_launch<BITS, EPI, 2, 3, 4, 2, BITS == kMx8 ? 3 : 5, 2>(a, splits, s); else break;
+    case 9: if constexpr (kGate) return mx_rows_launch<BITS, EPI, 4, 4>(a, splits, s); else break;
   }
   return static_cast<int>(hipErrorInvalidValue);
 }

@@ -315,7 +315,7 @@ def lay_weight(rows: MXRows, gated: bool = False) -> MXWeight:
 
 
 _EPI_F32, _EPI_GATE = F32, {"mxfp8": 2, "mxfp4": 3}                         # (sums leave as the type whose code this is)
-ROW_VARIANTS = (0, 1)                                                       # of up to 16 rows (mx_gemm_rows_kernel)
+ROW_VARIANTS, GATED_ROWS = (0, 1), 9                                        # of up to 16 rows (mx_gemm_rows_kernel), sums or gated
 # variant of mx_gemm_tiles_kernel -> rows, columns, workgroups a compute unit holds, us to start and end a launch, and us of 128 k for one workgroup
 # alone and for a compute unit that is as full as all others, for rows of 8 bits and of 4.  What they were read from (MI355X, us in a captured graph,
 # 2.4 of which are the launch; rows x N x K, 8 bits if not said):
@@ -371,6 +371,10 @@ def _choose(M: int, n_tiles: int, k_tiles: int, bits: int, gated: bool, whole: b
         if whole:
             return (0 if pairs >= 192 else 1), 1
         return 0, _even(min(max(1, round(640 / pairs)), 8, max(1, k_tiles // 4)), k_tiles)
+    if M <= 16 and n_tiles <= 1024:
+        # us, the few rows' kernel / tiles of 64 x 128, of which there are too few to fill the chip then: 8 x 1,024 x 4,096 6.6 / 10.6, 8 x 3,200 x 1,024 3.7 /
+        # 5.4, 16 x 6,144 x 2,048 6.1 / 8.0 (ff x K); 8 x 9,728 x 2,560 9.2 / 9.3, 16 rows 10.0 / 9.3, 8 x 12,288 x 4,096 13.5 / 12.7
+        return GATED_ROWS, 1
     found = []
     for variant in _TILES:
         if gated and variant in _PLAIN_TILES:
@@ -392,7 +396,7 @@ def _even(splits: int, steps: int) -> int:
 
 def _per_split(M: int, k_tiles: int, bits: int, variant: int, splits: int) -> int:
     """Steps of K that a part walks; refuses what the kernel was not written for."""
-    few = variant in ROW_VARIANTS
+    few = variant in ROW_VARIANTS or variant == GATED_ROWS
     if not few and variant not in _TILES:
         raise ShapeError(f"no variant {variant}")
     if few and M > 16:
@@ -438,6 +442,8 @@ def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partia
         variant, splits, per_split = _plan(M, n_tiles, k_tiles, bits, False, not partials_ok)
     else:
         splits = splits or 1
+        if variant == GATED_ROWS:
+            raise ShapeError(f"variant {variant} makes blocks")
         per_split = _per_split(M, k_tiles, bits, variant, splits)
     parts = splits > 1
     out = _empty(splits, M, N, dtype=torch.float32, device=on) if parts else _empty(M, N, dtype=out_dtype, device=on)

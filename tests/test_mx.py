@@ -193,10 +193,11 @@ def test_every_size_has_a_plan(bits, gated, whole):
         for n_tiles in (1, 3, 64, 96, 160, 384, 1216, 9496):
             for k_tiles in (4, 8, 20, 32, 76, 96, 1000):
                 variant, splits, per_split = mx._plan(M, n_tiles, k_tiles, bits, gated, whole)
-                steps = k_tiles if variant in mx.ROW_VARIANTS else k_tiles // 4
+                few = variant in (*mx.ROW_VARIANTS, mx.GATED_ROWS)
+                steps = k_tiles if few else k_tiles // 4
                 assert splits >= 1 and (splits - 1) * per_split < steps <= splits * per_split
-                assert M <= 16 if variant in mx.ROW_VARIANTS else variant in mx._TILES
-                assert not gated or (splits == 1 and variant in (3, 4, 5, 6))
+                assert M <= 16 if few else variant in mx._TILES
+                assert (splits == 1 and variant in (3, 4, 5, 6, mx.GATED_ROWS)) if gated else variant != mx.GATED_ROWS
 
 
 def test_no_rows_launch_nothing(no_gpu):
@@ -231,3 +232,11 @@ def test_designs_without_that_form_are_refused():
     other = detect_architecture(raw)
     with pytest.raises(EngineError, match="not built for"):
         engine._check_weight_form(other.recipe(other.config_class.from_dict(raw), ()), "mxfp4", "mxfp8")
+
+
+def test_few_gated_rows_have_a_kernel_of_their_own(no_gpu):
+    x, wg, w = _rows(3, 64)[2], mx.lay_weight(_rows(64, 64, "mxfp4")[2], gated=True), mx.lay_weight(_rows(64, 64, "mxfp4")[2])
+    assert mx._plan(16, wg.n_tiles, wg.k_tiles, 8, True, True)[0] == mx.GATED_ROWS and mx._plan(17, wg.n_tiles, wg.k_tiles, 8, True, True)[0] in mx._TILES
+    for call in (lambda: mx.gemm(x, w, variant=mx.GATED_ROWS), lambda: mx.gate_up_act(_rows(17, 64)[2], wg, variant=mx.GATED_ROWS)):
+        with pytest.raises(ops.ShapeError):
+            call()

@@ -210,6 +210,32 @@ def test_workgroups_with_several_tiles(form, K):
     assert torch.equal(parts.double().sum(0) if parts.dim() == 3 else parts.double(), want)
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("out", FORMS)
+@pytest.mark.parametrize("ff,K", [(1, 40), (32, 256), (100, 300), (700, 1100), (4000, 520)])
+def test_gated_products_of_few_rows(form, out, ff, K):
+    """The few rows' kernel against the tiles' one: whole numbers, whose sums are exact in any order, give the same blocks bit for bit; a block
+    that is no number in a row, and one in a column of each half, give none where they enter."""
+    few = torch.tensor([0, 2, 4, 5, 8, 10, 12, 13] if form == "mxfp4" else [0, 0x38, 0x40, 0x44, 0x80, 0xB8, 0xC0, 0xC4], dtype=torch.uint8)
+    for M in (1, 7, 16):
+        xe, we = few[torch.randint(0, 8, (M, K), generator=_g(M))], torch.randint(0, 16, (2 * ff, K), generator=_g(ff), dtype=torch.uint8)
+        xs, ws = (torch.randint(122, 125, (n, -(-K // 32)), generator=_g(n + 1), dtype=torch.uint8) for n in (M, 2 * ff))
+        for none in (False, True):
+            if none:
+                xs[M // 2, -1] = ws[ff // 2, 0] = ws[ff + ff // 3, -1] = 255
+            x = mx.rows_from_codes(xe.to(DEV), xs.to(DEV), K, form)
+            w = mx.lay_weight(mx.rows_from_codes(we.to(DEV), ws.to(DEV), K, "mxfp4"), gated=True)
+            want, got = plain.unpack(mx.gate_up_act(x, w, out, variant=3)), plain.unpack(mx.gate_up_act(x, w, out, variant=mx.GATED_ROWS))
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (M, none)
+            if not none:
+                xv, wv = plain.dequantize(xe, xs, form), plain.dequantize(we, ws, "mxfp4")
+                y, held = plain.gated(xv, wv), plain.dequantize(got[0][:, :ff], got[1][:, :-(-ff // 32)], out)
+                half, least = {"mxfp8": (2.0**-4, 2.0**-10), "mxfp4": (2.0**-2, 2.0**-2)}[out]
+                step = torch.maximum(half * y.abs(), least * plain.scale_values(got[1]).repeat_interleave(32, 1)[:, :ff])
+                assert ((held - y).abs() <= step * (1 + 2.0**-10) + 2.0**-18 * y.abs() + 2.0**-100).all()
+    assert all(torch.equal(a, b) for a, b in zip(plain.unpack(mx.gate_up_act(x, w, out)), plain.unpack(mx.gate_up_act(x, w, out, variant=mx.GATED_ROWS))))
+
+
 def _at_the_end(t):
     """The same numbers in the last bytes of an allocation that ends with its mapping (of its own, a multiple of 2 MiB): a kernel that reads past
     what it was given, wherever that is the last of it, does not get away with it."""
@@ -234,9 +260,10 @@ def test_operands_at_the_end_of_their_memory(form):
         for variant in range(9):
             if variant > 1 or M <= 16:
                 assert torch.equal(mx.gemm(x, ends[0], torch.float32, variant=variant), mx.gemm(rows, w, torch.float32, variant=variant)), (M, variant)
-        for variant in (3, 4, 5, 6):
-            got, want = mx.gate_up_act(x, ends[1], form, variant=variant), mx.gate_up_act(rows, wg, form, variant=variant)
-            assert all(torch.equal(a, b) for a, b in zip(plain.unpack(got), plain.unpack(want))), (M, variant)
+        for variant in (3, 4, 5, 6, mx.GATED_ROWS):
+            if variant != mx.GATED_ROWS or M <= 16:
+                got, want = mx.gate_up_act(x, ends[1], form, variant=variant), mx.gate_up_act(rows, wg, form, variant=variant)
+                assert all(torch.equal(a, b) for a, b in zip(plain.unpack(got), plain.unpack(want))), (M, variant)
         assert torch.equal(mx.values(x), mx.values(rows))
     for n in (1, 16, 100):      # fewer columns than a tile has
         few = mx.lay_weight(mx.quantize(torch.randn(n, K, generator=_g(n)).to(DEV), "mxfp4"))
