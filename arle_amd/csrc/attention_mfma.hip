@@ -32,6 +32,7 @@
 #include "attention_static.h"
 #include "attention_args.h"
 #include "attention_stream.h"
+#include "attention_blocks.h"
 #include "attention_portions.h"
 #include "attention_portions_dma.h"
 
@@ -486,13 +487,13 @@ void launch_decode_prep(const AttnArgs& a, bool whole_in, dim3 grid, int threads
 // window and waves with plan_made 1; without `waves` it is scratch of the call, which may leave it unwritten).  D 64 or 128, nq / nkv <= 16; everything else
 // as arle_attn_paged_mfma with max_qlen 1.  The same results as arle_qk_prep followed by arle_attn_paged_mfma but
 // for the order in which a head's squares are added for its norm.
-extern "C" int arle_attn_decode_prep(const void* parts, int parts_bf16, int n_parts, long long part_stride, long long row_stride,
+static int decode_prep(const void* parts, int parts_bf16, int n_parts, long long part_stride, long long row_stride,
                                      const void* q_w, const void* k_w, int w_f32, const float* cos_t, const float* sin_t,
                                      int rot, float eps, void* out, long long o_stride, void* k_pages, void* v_pages,
                                      const int* block_table, int table_stride, const int* seg_row0, const int* seg_slot,
                                      const int* seg_start, int segments, int nq, int nkv, int D, int page_size,
                                      float scale, int window, int splits, float* ws_o, float* ws_ml, int waves, int* ws_plan,
-                                     int plan_made, void* stream) {
+                                     int plan_made, const MergeBlocks* blocks, void* stream) {
   if (segments == 0) return 0;
   auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   if ((D != 64 && D != 128) || page_size < 4 || (page_size & (page_size - 1)) != 0 || nkv <= 0 || nq % nkv != 0 ||
@@ -524,13 +525,20 @@ extern "C" int arle_attn_decode_prep(const void* parts, int parts_bf16, int n_pa
   a.prep_eps = eps;
   a.prep_k_pages = static_cast<uint16_t*>(k_pages);
   a.prep_v_pages = static_cast<uint16_t*>(v_pages);
+  auto merge_blocks = [&](const float* o, const float* ml) {
+    const dim3 grid(segments, blocks->padded / D);
+    const auto kernel = blocks->bits == kMx8 ? attn_merge_blocks_kernel<kMx8> : attn_merge_blocks_kernel<kMx4>;
+    kernel<<<grid, kMergeWaves * kWave, 0, s>>>(o, ml, a.out, o_stride, seg_row0, nq, nkv, D, splits, a.sink, a.out_scale, a.ws_plan, *blocks);
+    return launch_status();
+  };
   // two to four splits and a workgroup for every compute unit even so: the splits of a (segment, kv head) share a
   // workgroup and merge in LDS (measured on MI355X at the Qwen3-4B widths, 64 requests at 2,048 tokens in two splits)
   if (!spread && splits > 1 && splits <= kInWgWavesMax && g_decode_inwg != 0 &&
       (g_decode_inwg > 0 || static_cast<long long>(segments) * nkv >= compute_units())) {
     const dim3 grid(1, nkv, static_cast<unsigned>(segments));
     launch_decode_prep<true>(a, parts_bf16 != 0, grid, splits * kWave, s);
-    return launch_status();
+    const int rc = launch_status();
+    return rc != 0 || blocks == nullptr ? rc : merge_blocks(nullptr, nullptr);
   }
   a.segments = segments;
   a.ws_plan = splits > 1 ? ws_plan : nullptr;
@@ -538,10 +546,41 @@ extern "C" int arle_attn_decode_prep(const void* parts, int parts_bf16, int n_pa
   const dim3 grid(1, nkv, static_cast<unsigned>(z));
   launch_decode_prep<false>(a, parts_bf16 != 0, grid, kWave, s);
   const int rc = launch_status();
-  if (rc != 0 || splits == 1) return rc;
+  if (rc != 0) return rc;
+  if (blocks != nullptr) return splits == 1 ? merge_blocks(nullptr, nullptr) : merge_blocks(ws_o, ws_ml);
+  if (splits == 1) return rc;
   attn_merge_kernel<<<dim3(segments * a.ws_rows, nq), kMergeWaves * kWave, 0, s>>>(
       ws_o, ws_ml, a.out, o_stride, seg_row0, a.ws_rows, 0, nq, nkv, D, splits, a.sink, a.out_scale, a.ws_plan);
   return launch_status();
+}
+
+extern "C" int arle_attn_decode_prep(const void* parts, int parts_bf16, int n_parts, long long part_stride, long long row_stride,
+                                     const void* q_w, const void* k_w, int w_f32, const float* cos_t, const float* sin_t,
+                                     int rot, float eps, void* out, long long o_stride, void* k_pages, void* v_pages,
+                                     const int* block_table, int table_stride, const int* seg_row0, const int* seg_slot,
+                                     const int* seg_start, int segments, int nq, int nkv, int D, int page_size,
+                                     float scale, int window, int splits, float* ws_o, float* ws_ml, int waves, int* ws_plan,
+                                     int plan_made, void* stream) {
+  return decode_prep(parts, parts_bf16, n_parts, part_stride, row_stride, q_w, k_w, w_f32, cos_t, sin_t, rot, eps, out, o_stride, k_pages,
+                     v_pages, block_table, table_stride, seg_row0, seg_slot, seg_start, segments, nq, nkv, D, page_size, scale, window, splits,
+                     ws_o, ws_ml, waves, ws_plan, plan_made, nullptr, stream);
+}
+
+// The same with the results in blocks besides (attention_blocks.h): elements [segments][padded] of `bits` bits, scales [segments][padded / 32],
+// padded the next multiple of 512 from nq D on.  `out` holds results or is left as it was, row by row.
+extern "C" int arle_attn_decode_prep_blocks(const void* parts, int parts_bf16, int n_parts, long long part_stride, long long row_stride,
+                                            const void* q_w, const void* k_w, int w_f32, const float* cos_t, const float* sin_t,
+                                            int rot, float eps, void* out, long long o_stride, void* k_pages, void* v_pages,
+                                            const int* block_table, int table_stride, const int* seg_row0, const int* seg_slot,
+                                            const int* seg_start, int segments, int nq, int nkv, int D, int page_size,
+                                            float scale, int window, int splits, float* ws_o, float* ws_ml, int waves, int* ws_plan,
+                                            int plan_made, void* elements, void* scales, int bits, int padded, void* stream) {
+  if ((bits != kMx8 && bits != kMx4) || padded % 512 != 0 || padded < nq * D || padded >= nq * D + 512 || elements == nullptr || scales == nullptr)
+    return static_cast<int>(hipErrorInvalidValue);
+  const MergeBlocks blocks = {static_cast<uint8_t*>(elements), static_cast<uint8_t*>(scales), bits, padded};
+  return decode_prep(parts, parts_bf16, n_parts, part_stride, row_stride, q_w, k_w, w_f32, cos_t, sin_t, rot, eps, out, o_stride, k_pages,
+                     v_pages, block_table, table_stride, seg_row0, seg_slot, seg_start, segments, nq, nkv, D, page_size, scale, window, splits,
+                     ws_o, ws_ml, waves, ws_plan, plan_made, &blocks, stream);
 }
 
 // ---- the entry point that allocates nothing (attention_static.h) ---------------------------------------------

@@ -654,10 +654,11 @@ __global__ __launch_bounds__(INWG ? kInWgWavesMax * kWave : kWave) void attn_mfm
 // number; a segment of one wave has its result already.
 constexpr int kMergeWaves = 4;
 constexpr int kMergeMaxD = 256;
-__global__ __launch_bounds__(kMergeWaves* kWave) void attn_merge_kernel(
-    const float* __restrict__ ws_o, const float* __restrict__ ws_ml, uint16_t* __restrict__ out,
-    int64_t o_stride, const int* __restrict__ seg_row0, int ws_rows, int rows_max, int nq, int nkv, int D,
-    int splits, const float* __restrict__ sink, float out_scale, const int* __restrict__ plan) {
+// leave(row, head, d0, four numbers) is called by the lanes of the first wave that own columns.
+template <typename Leave>
+__device__ __forceinline__ void attn_merge_body(const float* __restrict__ ws_o, const float* __restrict__ ws_ml, const int* __restrict__ seg_row0,
+                                                int ws_rows, int rows_max, int nq, int nkv, int D, int splits, const float* __restrict__ sink,
+                                                float out_scale, const int* __restrict__ plan, Leave leave) {
   __shared__ float part[kMergeWaves][kMergeMaxD];
   const int head = blockIdx.y;
   const int seg = blockIdx.x / ws_rows, tok = blockIdx.x % ws_rows;
@@ -722,11 +723,20 @@ __global__ __launch_bounds__(kMergeWaves* kWave) void attn_merge_kernel(
       o.z += p.z;
       o.w += p.w;
     }
-    uint2 w;
-    w.x = static_cast<uint32_t>(f32_to_bf16_bits(o.x * inv)) | (static_cast<uint32_t>(f32_to_bf16_bits(o.y * inv)) << 16);
-    w.y = static_cast<uint32_t>(f32_to_bf16_bits(o.z * inv)) | (static_cast<uint32_t>(f32_to_bf16_bits(o.w * inv)) << 16);
-    *reinterpret_cast<uint2*>(out + static_cast<int64_t>(row) * o_stride + head * D + d0) = w;
+    leave(row, head, d0, float4{o.x * inv, o.y * inv, o.z * inv, o.w * inv});
   }
+}
+
+__global__ __launch_bounds__(kMergeWaves* kWave) void attn_merge_kernel(
+    const float* __restrict__ ws_o, const float* __restrict__ ws_ml, uint16_t* __restrict__ out,
+    int64_t o_stride, const int* __restrict__ seg_row0, int ws_rows, int rows_max, int nq, int nkv, int D,
+    int splits, const float* __restrict__ sink, float out_scale, const int* __restrict__ plan) {
+  attn_merge_body(ws_o, ws_ml, seg_row0, ws_rows, rows_max, nq, nkv, D, splits, sink, out_scale, plan, [&](int row, int head, int d0, float4 o) {
+    uint2 w;
+    w.x = static_cast<uint32_t>(f32_to_bf16_bits(o.x)) | (static_cast<uint32_t>(f32_to_bf16_bits(o.y)) << 16);
+    w.y = static_cast<uint32_t>(f32_to_bf16_bits(o.z)) | (static_cast<uint32_t>(f32_to_bf16_bits(o.w)) << 16);
+    *reinterpret_cast<uint2*>(out + static_cast<int64_t>(row) * o_stride + head * D + d0) = w;
+  });
 }
 
 }  // namespace arle

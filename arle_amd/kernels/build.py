@@ -63,7 +63,7 @@ HEADERS = ("common.h", "once_a_device.h", "attention_static.h", "attention_args.
 # headers that only some sources include: they count for those alone, so that a change compiles no other library again
 # (the same with flags: "source" keeps a basic block in the order in which it is written, into which a loop's reads and products are woven by hand)
 OWN_FLAGS = {"mx_gemm": ["-mllvm", "-pre-RA-sched=source"]}
-OWN_HEADERS = {"mx_rows": ("mx.h",), "mx_gemm": ("mx.h",)}
+OWN_HEADERS = {"mx_rows": ("mx.h",), "mx_gemm": ("mx.h",), "attention_mfma": ("mx.h", "attention_blocks.h")}
 HOST_LIBS = ("host",)   # plain C++: page pool, block tables, step packing
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared"]
 

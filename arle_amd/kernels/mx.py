@@ -134,6 +134,14 @@ def _new_rows(rows: int, width: int, form: str, bits: int, device: int) -> MXRow
                          width, form, rows, padded, bits, device))
 
 
+def empty_rows(rows: int, width: int, form: str) -> MXRows:
+    """Rows that a kernel is to fill, on the current device."""
+    bits = _bits(form)
+    if rows < 0 or not 1 <= width <= MAX_K:
+        raise ShapeError(f"rows have 1 to {MAX_K} columns, got [{rows}, {width}]")
+    return _new_rows(rows, width, form, bits, _current())
+
+
 _DEVICES: dict = {}
 
 

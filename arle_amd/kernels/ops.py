@@ -564,7 +564,7 @@ def attn_decode_prep_supported(dtype, head_dim: int, page_size: int, group: int,
 def attn_decode_prep(parts, out, k_pages, v_pages, block_table, seg_row0, seg_slot, seg_start, *, max_kv_len: int,
                      num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, scale: float, eps: float,
                      q_weight=None, k_weight=None, cos=None, sin=None, rotary_dim: int = 0, window: int = 0,
-                     splits: int | None = None, total_kv_len: int | None = None, carry: dict | None = None):
+                     splits: int | None = None, total_kv_len: int | None = None, carry: dict | None = None, blocks=None):
     """A step of single decoded tokens (segment s is token row s) from the float32 stack of partial products
     [S, T, (nq + 2 nkv) D] of its fused q|k|v projection, or from the projection itself in bfloat16 [T, (nq + 2 nkv) D]:
     what qk_prep and attn_paged_mfma do one after the other, in the attention's own kernel.  Every wave sums, norms and rotates its q heads itself; the wave whose keys end
@@ -573,7 +573,8 @@ def attn_decode_prep(parts, out, k_pages, v_pages, block_table, seg_row0, seg_sl
     total_kv_len: the contexts' lengths together, by which ragged ones are told from equal ones (decode_share).
     carry: a dictionary that lives for one pass over the layers.  Where decode_share has the requests' keys shared out over all
     waves of a kv head, the first layer works out how, and the later ones of the pass with as many waves and the same
-    window find it there."""
+    window find it there.
+    blocks (mx.MXRows [T, nq*D] of their own): the results go there, as mx.quantize would make them, and `out` is scratch."""
     _gpu(parts, out, k_pages, v_pages, block_table, seg_row0, seg_slot, seg_start, q_weight, k_weight, cos, sin)
     group = num_q_heads // max(num_kv_heads, 1)
     width = (num_q_heads + 2 * num_kv_heads) * head_dim
@@ -633,12 +634,17 @@ def attn_decode_prep(parts, out, k_pages, v_pages, block_table, seg_row0, seg_sl
         if not plan_made:
             kept[key] = torch.empty((2 * segments + 8 * held,), dtype=torch.int32, device=out.device)
         plan = kept[key]
-    lib.call("arle_attn_decode_prep", parts.data_ptr(), int(whole), n_parts, part_stride, row_stride, _ptr(q_weight),
+    name, more = "arle_attn_decode_prep", ()
+    if blocks is not None:
+        _need((blocks.rows, blocks.width) == (tokens, num_q_heads * head_dim) and blocks.elements.is_contiguous() and blocks.scales.is_contiguous()
+              and blocks.device == out.get_device(), "blocks must be contiguous rows [T, nq*D] on the same device")
+        name, more = "arle_attn_decode_prep_blocks", (blocks.elements.data_ptr(), blocks.scales.data_ptr(), blocks.bits, blocks.padded)
+    lib.call(name, parts.data_ptr(), int(whole), n_parts, part_stride, row_stride, _ptr(q_weight),
              _ptr(k_weight), w_f32, _ptr(cos), _ptr(sin), int(rotary_dim), float(eps), out.data_ptr(), out.stride(0),
              k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), block_table.shape[1], seg_row0.data_ptr(),
              seg_slot.data_ptr(), seg_start.data_ptr(), segments, num_q_heads, num_kv_heads, head_dim, page_size,
-             float(scale), int(window), int(splits), _ptr(ws_o), _ptr(ws_ml), int(waves), _ptr(plan), int(plan_made), _stream())
-    return out
+             float(scale), int(window), int(splits), _ptr(ws_o), _ptr(ws_ml), int(waves), _ptr(plan), int(plan_made), *more, _stream())
+    return out if blocks is None else blocks
 
 
 _plan_tokens = itertools.count(1)

@@ -157,12 +157,14 @@ class PagedAttention(Part):
                 and ops.attn_decode_prep_supported(dtype, self.D, cache.page_size, self.nq // self.nkv, rot)):
             # single decoded tokens: the attention's kernel sums, norms, rotates and writes to the cache itself
             out = torch.empty((rows, Q), dtype=dtype, device=device)
-            ops.attn_decode_prep(projected, out, cache.k_pages, cache.v_pages, cache.block_table, batch.seg_row0,
-                                 batch.seg_slot, batch.seg_start, max_kv_len=batch.max_position + 1,
-                                 num_q_heads=self.nq, num_kv_heads=self.nkv, head_dim=self.D, page_size=cache.page_size,
-                                 scale=self.scale, eps=self.eps, q_weight=self.q_norm, k_weight=self.k_norm, cos=cos,
-                                 sin=sin, rotary_dim=rot, window=self.window or 0, splits=getattr(batch, "kv_splits", None),
-                                 total_kv_len=getattr(batch, "total_context", 0) or None, carry=getattr(batch, "carry", None))
+            blocks = mx.empty_rows(rows, Q, self.rt.row_form) if self.rt.weight_form else None
+            out = ops.attn_decode_prep(projected, out, cache.k_pages, cache.v_pages, cache.block_table, batch.seg_row0,
+                                       batch.seg_slot, batch.seg_start, max_kv_len=batch.max_position + 1,
+                                       num_q_heads=self.nq, num_kv_heads=self.nkv, head_dim=self.D, page_size=cache.page_size,
+                                       scale=self.scale, eps=self.eps, q_weight=self.q_norm, k_weight=self.k_norm, cos=cos,
+                                       sin=sin, rotary_dim=rot, window=self.window or 0, splits=getattr(batch, "kv_splits", None),
+                                       total_kv_len=getattr(batch, "total_context", 0) or None, carry=getattr(batch, "carry", None),
+                                       blocks=blocks)
             return self.o.late(out) if late and self.leaves_late else self.o(out, partials_ok=True)
         if projected.dim() == 3:
             q = torch.empty((rows, Q), dtype=dtype, device=device)

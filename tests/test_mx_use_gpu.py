@@ -277,3 +277,46 @@ def test_operands_at_the_end_of_their_memory(form):
         a = mx.add_rmsnorm(_at_the_end(residual), _at_the_end(torch.stack([numbers, numbers])), weight, 1e-6, form)
         b = mx.add_rmsnorm(residual, torch.stack([numbers, numbers]), weight, 1e-6, form)
         assert all(torch.equal(p, q) for p, q in zip(plain.unpack(a), plain.unpack(b)))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("D,nq,nkv", [(128, 32, 8), (128, 6, 2), (64, 12, 4), (64, 32, 8)])
+@pytest.mark.parametrize("contexts", [[0], [2047], [31, 32, 700, 0, 63], [900] * 9, [3000] + [40] * 40])
+def test_attention_that_leaves_blocks(form, D, nq, nkv, contexts):
+    """A step of decoded tokens whose results leave in blocks, bit for bit those that quantize makes of the same step's: splits that are merged
+    by a kernel, or inside a workgroup, or one wave a request, and shared-out keys with some requests of one wave."""
+    from arle_amd.kernels import lib, ops
+
+    P, T = 16, len(contexts)
+    pages = [(c + 1 + P - 1) // P for c in contexts]
+    order = torch.randperm(sum(pages), generator=_g(1)).to(torch.int32)
+    table = torch.zeros(T, max(pages), dtype=torch.int32)
+    for i, part in enumerate(order.split(pages)):
+        table[i, :len(part)] = part
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    k, v = (torch.randn(sum(pages), nkv, *shape, generator=_g(2)).bfloat16().to(DEV) for shape in ((P, D), (D, P)))
+    parts = torch.randn(2, T, (nq + 2 * nkv) * D, generator=_g(3)).to(DEV)
+
+    def run(inwg=-1, **kw):
+        out = torch.zeros(T, nq * D, dtype=torch.bfloat16, device=DEV)
+        lib.function("arle_attn_decode_inwg")(inwg)
+        try:
+            return ops.attn_decode_prep(parts, out, k.clone(), v.clone(), table.to(DEV), i32(list(range(T + 1))), i32(list(range(T))), i32(contexts),
+                                        max_kv_len=max(contexts) + 1, num_q_heads=nq, num_kv_heads=nkv, head_dim=D, page_size=P, scale=D**-0.5,
+                                        eps=1e-6, **kw)
+        finally:
+            lib.function("arle_attn_decode_inwg")(-1)
+
+    for kw in (dict(splits=1), dict(splits=5), dict(splits=2, inwg=1), dict(splits=2, inwg=0), dict(total_kv_len=sum(contexts) + T), dict()):
+        want = mx.quantize(run(**kw), form)
+        blocks = mx.empty_rows(T, nq * D, form)
+        blocks.elements.view(torch.uint8).fill_(0x77)
+        blocks.scales.view(torch.uint8).fill_(0x77)
+        got = run(blocks=blocks, **kw)
+        assert got is blocks and _same_rows(got, want), kw
+    with pytest.raises(ops.ShapeError):
+        run(blocks=mx.empty_rows(T, nq * D + 32, form))
+
+
+def _same_rows(a, b):
+    return a[2:5] == b[2:5] and all(torch.equal(p, q) for p, q in zip(plain.unpack(a), plain.unpack(b)))
