@@ -636,8 +636,8 @@ def attn_decode_prep(parts, out, k_pages, v_pages, block_table, seg_row0, seg_sl
         plan = kept[key]
     name, more = "arle_attn_decode_prep", ()
     if blocks is not None:
-        _need((blocks.rows, blocks.width) == (tokens, num_q_heads * head_dim) and blocks.elements.is_contiguous() and blocks.scales.is_contiguous()
-              and blocks.device == out.get_device(), "blocks must be contiguous rows [T, nq*D] on the same device")
+        _need(hasattr(blocks, "padded") and (blocks.rows, blocks.width) == (tokens, num_q_heads * head_dim) and blocks.elements.is_contiguous()
+              and blocks.scales.is_contiguous() and blocks.device == out.get_device(), "blocks must be contiguous mx.MXRows [T, nq*D] on the same device")
         name, more = "arle_attn_decode_prep_blocks", (blocks.elements.data_ptr(), blocks.scales.data_ptr(), blocks.bits, blocks.padded)
     lib.call(name, parts.data_ptr(), int(whole), n_parts, part_stride, row_stride, _ptr(q_weight),
              _ptr(k_weight), w_f32, _ptr(cos), _ptr(sin), int(rotary_dim), float(eps), out.data_ptr(), out.stride(0),

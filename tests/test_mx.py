@@ -240,3 +240,37 @@ def test_few_gated_rows_have_a_kernel_of_their_own(no_gpu):
     for call in (lambda: mx.gemm(x, w, variant=mx.GATED_ROWS), lambda: mx.gate_up_act(_rows(17, 64)[2], wg, variant=mx.GATED_ROWS)):
         with pytest.raises(ops.ShapeError):
             call()
+
+
+def test_empty_rows(no_gpu):
+    for form in ("mxfp8", "mxfp4"):
+        rows = mx.empty_rows(5, 700, form)
+        again = mx.MXRows(rows.elements, rows.scales, 700, form)      # as a user would make them, checked
+        assert rows[2:] == again[2:] and rows.rows == 5 and rows.elements.is_contiguous()
+    for args in ((5, 0, "mxfp8"), (-1, 32, "mxfp8"), (5, 32, "fp8"), (5, mx.MAX_K + 1, "mxfp4")):
+        with pytest.raises(ops.ShapeError):
+            mx.empty_rows(*args)
+
+
+def test_blocks_that_attention_cannot_fill(no_gpu, monkeypatch):
+    monkeypatch.setattr(ops, "_gpu", lambda *tensors: None)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    calls = []
+    monkeypatch.setattr(ops.lib, "call", lambda name, *args: calls.append((name, args)))
+    i32 = lambda values: torch.tensor(list(values), dtype=torch.int32)
+
+    def run(blocks):
+        out = torch.zeros(3, 8 * 64, dtype=torch.bfloat16)
+        return ops.attn_decode_prep(torch.zeros(2, 3, 12 * 64), out, torch.zeros(6, 2, 16, 64, dtype=torch.bfloat16),
+                                    torch.zeros(6, 2, 64, 16, dtype=torch.bfloat16), torch.zeros(3, 2, dtype=torch.int32), i32(range(4)), i32(range(3)),
+                                    i32([20] * 3), max_kv_len=21, num_q_heads=8, num_kv_heads=2, head_dim=64, page_size=16, scale=1.0, eps=1e-6,
+                                    splits=1, blocks=blocks)
+
+    rows = mx.empty_rows(3, 512, "mxfp8")._replace(device=-1)      # the device number of a tensor on the host
+    assert run(rows) is rows and calls[-1][0] == "arle_attn_decode_prep_blocks" and calls[-1][1][-3:-1] == (8, 512)
+    assert run(None).shape == (3, 512) and calls[-1][0] == "arle_attn_decode_prep"
+    wide = mx.empty_rows(3, 1024, "mxfp8")
+    apart = rows._replace(elements=wide.elements[:, :512])
+    for bad in (rows._replace(rows=4), rows._replace(width=500), apart, rows._replace(device=0), rows.elements):
+        with pytest.raises(ops.ShapeError):
+            run(bad)
