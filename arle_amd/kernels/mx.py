@@ -102,7 +102,8 @@ class MXRows(_Rows):
                 and tuple(s.shape) == (e.shape[0], padded // BLOCK)):
             raise ShapeError(f"{form} rows of {width} are {_ELEMENTS[form]} [T, {padded * bits // 8}] with scales {_SCALES} [T, {padded // BLOCK}], got "
                              f"{e.dtype} {tuple(e.shape)} with {s.dtype} {tuple(s.shape)}")
-        if e.stride(1) != 1 or s.stride(1) != 1 or e.data_ptr() % 16 or s.data_ptr() % 16 or (e.shape[0] > 1 and (e.stride(0) % 16 or s.stride(0) % 16 or max(e.stride(0), s.stride(0)) > 2 * MAX_K)):
+        if (e.stride(1) != 1 or s.stride(1) != 1 or e.data_ptr() % 16 or s.data_ptr() % 16
+                or (e.shape[0] > 1 and (e.stride(0) % 16 or s.stride(0) % 16 or max(e.stride(0), s.stride(0)) > 2 * MAX_K))):
             raise ShapeError(f"rows of elements and scales must lie together and start at multiples of 16 bytes, up to {2 * MAX_K} apart")
         return tuple.__new__(cls, (e, s, int(width), form, e.shape[0], padded, bits, device))
 
@@ -267,8 +268,8 @@ _Weight = collections.namedtuple("_Weight", "tiles scales n k gated n_tiles k_ti
 
 class MXWeight(_Weight):
     """A weight [n, k] in 4 bits, laid out for the products (see lay_weight).  tiles uint8 [tiles of 128 k, tiles of 16 rows, 64, 16], scales uint8
-    [groups of 512 k, tiles of 16 rows, 64, 4]; both may be the first rows' tiles of a larger weight.  gated: n = 2 * ff rows, the gate's and then the up's, held in turns of 16 with both
-    halves padded with zeros to a multiple of 512."""
+    [groups of 512 k, tiles of 16 rows, 64, 4]; both may be the first rows' tiles of a larger weight.  gated: n = 2 * ff rows, the gate's and then
+    the up's, held in turns of 16 with both halves padded with zeros to a multiple of 512."""
     __slots__ = ()
 
     def __new__(cls, tiles: torch.Tensor, scales: torch.Tensor, n: int, k: int, gated: bool = False):
