@@ -274,3 +274,11 @@ def test_blocks_that_attention_cannot_fill(no_gpu, monkeypatch):
     for bad in (rows._replace(rows=4), rows._replace(width=500), apart, rows._replace(device=0), rows.elements):
         with pytest.raises(ops.ShapeError):
             run(bad)
+
+
+def test_views_without_the_padding(no_gpu):
+    e, s, rows = _rows(9, 700)
+    for part in (rows, rows.part(2, 7), rows.part(4, 4), mx.MXRows(rows.elements[1::3], rows.scales[1::3], 700, "mxfp8")):
+        a, b = part.elements_e4m3(), part.scales_e8m0()
+        assert torch.equal(a.view(torch.uint8), part.elements[:, :700].view(torch.uint8)) and a.data_ptr() == part.elements.data_ptr()
+        assert torch.equal(b.view(torch.uint8), part.scales[:, :22].view(torch.uint8)) and b.shape == (part.rows, 22)
