@@ -474,11 +474,9 @@ __global__ __launch_bounds__(RW* CW* kWave, WAVES_A_SIMD) void mx_gemm_tiles_ker
     };
     if constexpr (kGate) {
       constexpr int kBits = EPI == kMxGate8 ? kMx8 : kMx4;
-      // (whole blocks: the columns are a multiple of 512)
-      const int row_tiles = n_here / 16 < a.n_tiles ? MT : 0;
+      static_assert(64 % kTiles == 0, "whole blocks: a gated weight's tiles are a multiple of 64");
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        if (t >= row_tiles) break;
         const int row0 = m_here + 32 * (MT * wr + t);
         uint32_t packed[TN / 2][2][2];
 #pragma unroll
