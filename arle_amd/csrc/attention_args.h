@@ -56,6 +56,10 @@ struct AttnArgs {
   float prep_eps;
   uint16_t* prep_k_pages;  // the pages again, to write the new token's key and value into
   uint16_t* prep_v_pages;
+  // The portions kernel of head_dim 128: where results go in blocks of 32 instead of to `out` (attention_blocks.h); null: to `out`
+  uint8_t* blocks;
+  uint8_t* block_scales;
+  int block_bits;
 };
 
 __device__ __forceinline__ bf16x8 load_bf16x8(const uint16_t* p) {

@@ -272,6 +272,7 @@ static AttnArgs make_args(const void* q, long long q_stride, void* out, long lon
                           const int* seg_slot, const int* seg_start, int max_qlen, int nq, int nkv, int D,
                           int page_size, float scale, int window, int splits, float* ws_o, float* ws_ml) {
   AttnArgs a;
+  a.blocks = nullptr;
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride = q_stride;
   a.out = static_cast<uint16_t*>(out);
@@ -333,15 +334,15 @@ static AttnArgs make_args(const void* q, long long q_stride, void* out, long lon
 // sink: float32 [nq] or null; out_scale: a factor on the output (see AttnArgs).  short_segments: how many segments have
 // 16 rows at most, as far as the caller knows (choices of launches only).
 // Requires D % 16 == 0, D <= 256, page_size a power of two >= 4; rows of out 8-byte aligned.
-extern "C" int arle_attn_paged_mfma(const void* q, long long q_stride, void* out, long long o_stride,
-                                    const void* k_pages, const void* v_pages, const int* block_table,
-                                    int table_stride, const int* seg_row0, const int* seg_slot,
-                                    const int* seg_start, int segments, int max_qlen, int min_qlen,
-                                    int max_kv_len, int token_rows,
-                                    int nq, int nkv, int D, int page_size, float scale, int window,
-                                    int splits, float* ws_o, float* ws_ml, int portion_splits, float* pws_o,
-                                    float* pws_ml, long long plan_token, const float* sink, float out_scale,
-                                    int short_segments, void* stream) {
+static int paged_mfma(const void* q, long long q_stride, void* out, long long o_stride,
+                      const void* k_pages, const void* v_pages, const int* block_table,
+                      int table_stride, const int* seg_row0, const int* seg_slot,
+                      const int* seg_start, int segments, int max_qlen, int min_qlen,
+                      int max_kv_len, int token_rows,
+                      int nq, int nkv, int D, int page_size, float scale, int window,
+                      int splits, float* ws_o, float* ws_ml, int portion_splits, float* pws_o,
+                      float* pws_ml, long long plan_token, const float* sink, float out_scale,
+                      int short_segments, const MergeBlocks* blocks, void* stream) {
   if (segments == 0 || token_rows == 0) return 0;
   if (D % 16 != 0 || D > 256 || D <= 0 || page_size < 4 || (page_size & (page_size - 1)) != 0 || nq % nkv != 0 ||
       splits < 1 || splits > 64 || portion_splits < 1 || portion_splits > kPortionPartsMax ||
@@ -368,6 +369,12 @@ extern "C" int arle_attn_paged_mfma(const void* q, long long q_stride, void* out
     // step) through the streaming kernel
     dim3 grid((max_rows + kPfRows - 1) / kPfRows, nkv, segments);
     const bool dma = D == 128 && page_size % 8 == 0 && static_cast<long long>(nkv) * page_size * D < (1LL << 31) && g_prefill_dma != 0;
+    if (blocks != nullptr) {
+      if (!dma || min_rows <= 16 || portion_splits != 1) return static_cast<int>(hipErrorInvalidValue);
+      a.blocks = blocks->elements;
+      a.block_scales = blocks->scales;
+      a.block_bits = blocks->bits;
+    }
     if (dma && min_rows <= 16) {
       a.rows_max = 16;
       rc = launch_prefill_beside(a, grid, 17, splits, segments - short_segments, max_kv_len, s);
@@ -430,6 +437,7 @@ extern "C" int arle_attn_paged_mfma(const void* q, long long q_stride, void* out
         ws_o, ws_ml, a.out, o_stride, seg_row0, a.ws_rows, a.rows_max, nq, nkv, D, splits, a.sink, a.out_scale, a.ws_plan);
     return launch_status();
   }
+  if (blocks != nullptr) return static_cast<int>(hipErrorInvalidValue);
   if (max_rows > 16 && splits > 1) return static_cast<int>(hipErrorInvalidValue);  // two row tiles: no split
   // one row tile of 16 when a segment's rows fit it (decoded tokens), else two
   const int nt = max_rows <= 16 ? 1 : 2;
@@ -439,6 +447,39 @@ extern "C" int arle_attn_paged_mfma(const void* q, long long q_stride, void* out
   attn_merge_kernel<<<dim3(segments * a.ws_rows, nq), kMergeWaves * kWave, 0, s>>>(
       ws_o, ws_ml, a.out, o_stride, seg_row0, a.ws_rows, 0, nq, nkv, D, splits, a.sink, a.out_scale, a.ws_plan);
   return launch_status();
+}
+
+extern "C" int arle_attn_paged_mfma(const void* q, long long q_stride, void* out, long long o_stride,
+                                    const void* k_pages, const void* v_pages, const int* block_table,
+                                    int table_stride, const int* seg_row0, const int* seg_slot,
+                                    const int* seg_start, int segments, int max_qlen, int min_qlen,
+                                    int max_kv_len, int token_rows,
+                                    int nq, int nkv, int D, int page_size, float scale, int window,
+                                    int splits, float* ws_o, float* ws_ml, int portion_splits, float* pws_o,
+                                    float* pws_ml, long long plan_token, const float* sink, float out_scale,
+                                    int short_segments, void* stream) {
+  return paged_mfma(q, q_stride, out, o_stride, k_pages, v_pages, block_table, table_stride, seg_row0, seg_slot, seg_start, segments,
+                    max_qlen, min_qlen, max_kv_len, token_rows, nq, nkv, D, page_size, scale, window, splits, ws_o, ws_ml, portion_splits,
+                    pws_o, pws_ml, plan_token, sink, out_scale, short_segments, nullptr, stream);
+}
+
+// The same with the results in blocks (attention_blocks.h) instead of in `out`, for steps that are portions only (more than 16 rows each) with whole keys
+// (portion_splits 1) at head_dim 128, rows of a multiple of 512 columns: elements [token rows][nq D] of `bits` bits, scales [token rows][nq D / 32].
+extern "C" int arle_attn_paged_mfma_blocks(const void* q, long long q_stride, void* out, long long o_stride,
+                                           const void* k_pages, const void* v_pages, const int* block_table,
+                                           int table_stride, const int* seg_row0, const int* seg_slot,
+                                           const int* seg_start, int segments, int max_qlen, int min_qlen,
+                                           int max_kv_len, int token_rows,
+                                           int nq, int nkv, int D, int page_size, float scale, int window,
+                                           int splits, float* ws_o, float* ws_ml, int portion_splits, float* pws_o,
+                                           float* pws_ml, long long plan_token, const float* sink, float out_scale,
+                                           int short_segments, void* elements, void* scales, int bits,
+                                           void* stream) {
+  if ((bits != kMx8 && bits != kMx4) || elements == nullptr || scales == nullptr || nq * D % 512 != 0) return static_cast<int>(hipErrorInvalidValue);
+  const MergeBlocks blocks = {static_cast<uint8_t*>(elements), static_cast<uint8_t*>(scales), bits, nq * D};
+  return paged_mfma(q, q_stride, out, o_stride, k_pages, v_pages, block_table, table_stride, seg_row0, seg_slot, seg_start, segments,
+                    max_qlen, min_qlen, max_kv_len, token_rows, nq, nkv, D, page_size, scale, window, splits, ws_o, ws_ml, portion_splits,
+                    pws_o, pws_ml, plan_token, sink, out_scale, short_segments, &blocks, stream);
 }
 
 static int g_decode_inwg = -1;   // the splits of a decode step inside one workgroup: -1 by the rule, 0 never, 1 whenever they fit

@@ -485,14 +485,22 @@ __global__ __launch_bounds__(GROUPS* kDmWaves* kWave, GROUPS == 1 ? 2 : 1) void 
       const float inv_l = row_factor(a.sink, a.out_scale, my_head, m, l);
       uint16_t* op = a.out + static_cast<int64_t>(row0 + my_tok) * a.o_stride + my_head * D;
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
+      for (int dt = 0; dt < D / 32; ++dt) {
+        uint2 w[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          uint2 w;
-          w.x = pack_bf16x2(o[dt][4 * q] * inv_l, o[dt][4 * q + 1] * inv_l);
-          w.y = pack_bf16x2(o[dt][4 * q + 2] * inv_l, o[dt][4 * q + 3] * inv_l);
-          *reinterpret_cast<uint2*>(op + 32 * dt + 8 * q + 4 * h) = w;
+          w[q].x = pack_bf16x2(o[dt][4 * q] * inv_l, o[dt][4 * q + 1] * inv_l);
+          w[q].y = pack_bf16x2(o[dt][4 * q + 2] * inv_l, o[dt][4 * q + 3] * inv_l);
         }
+        if (a.blocks == nullptr) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) *reinterpret_cast<uint2*>(op + 32 * dt + 8 * q + 4 * h) = w[q];
+        } else if (a.block_bits == kMx8) {
+          leave_block<kMx8>(a, row0 + my_tok, my_head * D + 32 * dt, h, w);
+        } else {
+          leave_block<kMx4>(a, row0 + my_tok, my_head * D + 32 * dt, h, w);
+        }
+      }
     }
   }
  }  // next item

@@ -88,7 +88,7 @@ class Engine:
         weight_form: "mxfp4" holds the projections of attention and feed-forward in 4 bits, blocks of 32 numbers along
             the input with a power of two each (4.25 bits a weight), made from the checkpoint's weights when the engine is built;
             norms, embedding, head, cache and attention stay as they are.  The rows that meet them are made into blocks by the kernel in front
-            (norm, activation, the merge of a decode step's attention) as `row_form` says: "mxfp8" (e4m3) or "mxfp4".  For designs whose mixers and feed-forwards have
+            (norm, activation, attention) as `row_form` says: "mxfp8" (e4m3) or "mxfp4".  For designs whose mixers and feed-forwards have
             that form (the Qwen3 dense decoder), in bfloat16.  None: as the checkpoint holds them.
         weight_tiles: hold every bfloat16 projection weight a second time in the layout that the few-rows
             kernels stream fastest (decode steps about a tenth faster, twice the weight memory), and the projections

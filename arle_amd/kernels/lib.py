@@ -55,6 +55,8 @@ SIGNATURES = {
     "arle_attn_side_branch": ("attention_mfma", [_i]),
     "arle_attn_paged_mfma": ("attention_mfma", [_p, _ll, _p, _ll, _p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i,
                                                 _i, _i, _i, _f, _i, _i, _p, _p, _i, _p, _p, _ll, _p, _f, _i, _p]),
+    "arle_attn_paged_mfma_blocks": ("attention_mfma", [_p, _ll, _p, _ll, _p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i,
+                                                       _i, _i, _i, _f, _i, _i, _p, _p, _i, _p, _p, _ll, _p, _f, _i, _p, _p, _i, _p]),
     "arle_argmax_chunks": ("sampling", [_i, _i]),
     "arle_argmax_rows": ("sampling", [_p, _i, _i, _p, _p, _p]),
     "arle_sample_scratch_bytes": ("sampling", [_i, _i, _i]),

@@ -474,7 +474,7 @@ def attn_paged_mfma(q, out, k_pages, v_pages, block_table, seg_row0, seg_slot, s
                     max_qlen: int, max_kv_len: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
                     page_size: int, scale: float, window: int = 0, splits: int | None = None,
                     min_qlen: int = 1, short_segments: int | None = None, portion_splits: int | None = None,
-                    plan_token: int = 0, max_portion_kv_len: int | None = None, sink=None, out_scale: float = 1.0):
+                    plan_token: int = 0, max_portion_kv_len: int | None = None, sink=None, out_scale: float = 1.0, blocks=None):
     """Causal attention of a packed step on the matrix cores (bfloat16).
 
     Segments: rows seg_row0[s]..seg_row0[s+1] belong to block-table row seg_slot[s] and start at
@@ -489,6 +489,9 @@ def attn_paged_mfma(q, out, k_pages, v_pages, block_table, seg_row0, seg_slot, s
     the portions kernels plan by, so that a fresh portion beside requests that decode deep into their contexts is
     not cut into parts for the decoders' sake.  `sink` float32 [q heads]: exp(sink_h) joins the softmax's denominator;
     `out_scale`: a factor on the output, in 32 bits.  out may be a view whose rows lie further apart.
+    `blocks` (mx.MXRows [T, nq*D] of their own): where the portions kernel of head_dim 128 writes every row (portions only, with whole keys,
+    rows of a multiple of 512 columns), the results go there, as mx.quantize would make them, and not to `out`; the one of the two that
+    has them is returned.
     """
     _gpu(q, out, k_pages, v_pages, block_table, seg_row0, seg_slot, seg_start, sink)
     _need(sink is None or (sink.shape == (num_q_heads,) and sink.dtype == torch.float32 and sink.is_contiguous()),
@@ -541,14 +544,25 @@ def attn_paged_mfma(q, out, k_pages, v_pages, block_table, seg_row0, seg_slot, s
     if portion_splits > 1:
         pws_o = torch.empty((tokens, num_q_heads, portion_splits, head_dim), dtype=torch.float32, device=q.device)
         pws_ml = torch.empty((tokens, num_q_heads, portion_splits, 2), dtype=torch.float32, device=q.device)
-    lib.call("arle_attn_paged_mfma", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0),
+    name, more = "arle_attn_paged_mfma", ()
+    if blocks is not None:
+        _need_blocks(blocks, tokens, num_q_heads * head_dim, q)
+        if (head_dim == 128 and min_qlen * group > _ATTN_ROW_TILE and portion_splits == 1 and page_size % 8 == 0
+                and num_kv_heads * page_size * head_dim < 2**31 and blocks.padded == blocks.width):
+            name, more = "arle_attn_paged_mfma_blocks", (blocks.elements.data_ptr(), blocks.scales.data_ptr(), blocks.bits)
+    lib.call(name, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0),
              k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), block_table.shape[1],
              seg_row0.data_ptr(), seg_slot.data_ptr(), seg_start.data_ptr(), segments, int(max_qlen),
              int(min_qlen), int(max_portion_kv_len or max_kv_len), tokens,
              num_q_heads, num_kv_heads, head_dim, page_size, float(scale), int(window), int(splits),
              _ptr(ws_o), _ptr(ws_ml), int(portion_splits), _ptr(pws_o), _ptr(pws_ml), int(plan_token),
-             _ptr(sink), float(out_scale), min(short_segments or 0, segments), _stream())
-    return out
+             _ptr(sink), float(out_scale), min(short_segments or 0, segments), *more, _stream())
+    return blocks if more else out
+
+
+def _need_blocks(blocks, rows: int, width: int, like) -> None:
+    _need(hasattr(blocks, "padded") and (blocks.rows, blocks.width) == (rows, width) and blocks.elements.is_contiguous()
+          and blocks.scales.is_contiguous() and blocks.device == like.get_device(), "blocks must be contiguous mx.MXRows [T, nq*D] on the same device")
 
 
 _PREP_HEAD_DIMS = (64, 128)
@@ -636,8 +650,7 @@ def attn_decode_prep(parts, out, k_pages, v_pages, block_table, seg_row0, seg_sl
         plan = kept[key]
     name, more = "arle_attn_decode_prep", ()
     if blocks is not None:
-        _need(hasattr(blocks, "padded") and (blocks.rows, blocks.width) == (tokens, num_q_heads * head_dim) and blocks.elements.is_contiguous()
-              and blocks.scales.is_contiguous() and blocks.device == out.get_device(), "blocks must be contiguous mx.MXRows [T, nq*D] on the same device")
+        _need_blocks(blocks, tokens, num_q_heads * head_dim, out)
         name, more = "arle_attn_decode_prep_blocks", (blocks.elements.data_ptr(), blocks.scales.data_ptr(), blocks.bits, blocks.padded)
     lib.call(name, parts.data_ptr(), int(whole), n_parts, part_stride, row_stride, _ptr(q_weight),
              _ptr(k_weight), w_f32, _ptr(cos), _ptr(sin), int(rotary_dim), float(eps), out.data_ptr(), out.stride(0),

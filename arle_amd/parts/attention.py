@@ -187,28 +187,30 @@ class PagedAttention(Part):
                 if to_cache:
                     ops.qk_prep(q, k, v, **to_cache, **common)
         out = torch.empty((rows, Q), dtype=q.dtype, device=q.device)
-        paged_attention(q, out, cache, batch, num_q_heads=self.nq, num_kv_heads=self.nkv,
-                        head_dim=self.D, scale=self.scale, window=self.window or 0)
+        out = paged_attention(q, out, cache, batch, num_q_heads=self.nq, num_kv_heads=self.nkv,
+                              head_dim=self.D, scale=self.scale, window=self.window or 0, form=self.rt.row_form if self.rt.weight_form else None)
         return self.o.late(out) if late and self.leaves_late else self.o(out, partials_ok=True)
 
 
-def paged_attention(q, out, cache, batch, *, num_q_heads, num_kv_heads, head_dim, scale, window):
-    """Attention of every row of the packed step over its request's cached keys.
+def paged_attention(q, out, cache, batch, *, num_q_heads, num_kv_heads, head_dim, scale, window, form=None):
+    """Attention of every row of the packed step over its request's cached keys; returns `out`, or with `form` possibly the results in
+    blocks of that form (mx.MXRows).
 
     bfloat16 storage runs the matrix-core kernel (split over the keys when the step holds only
     single decoded tokens); float32 storage, and shapes the matrix-core kernel does not take,
     run the fixed-order kernel, which is also the true 32-bit path.
     """
     if ops.attn_mfma_supported(q.dtype, head_dim, cache.page_size):
-        ops.attn_paged_mfma(q, out, cache.k_pages, cache.v_pages, cache.block_table, batch.seg_row0,
-                            batch.seg_slot, batch.seg_start, max_qlen=batch.max_qlen, min_qlen=batch.min_qlen,
-                            max_kv_len=batch.max_position + 1, num_q_heads=num_q_heads,
-                            num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=cache.page_size,
-                            scale=scale, window=window, splits=getattr(batch, "kv_splits", None),
-                            short_segments=getattr(batch, "single_segments", 0) or None,
-                            plan_token=getattr(batch, "plan_token", 0),
-                            max_portion_kv_len=getattr(batch, "max_portion_kv", 0) or None)
-    else:
-        ops.attn_paged_simt(q, out, cache.k_pages, cache.v_pages, cache.block_table, batch.positions,
-                            batch.slot_of_token, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,
-                            head_dim=head_dim, page_size=cache.page_size, scale=scale, window=window)
+        return ops.attn_paged_mfma(q, out, cache.k_pages, cache.v_pages, cache.block_table, batch.seg_row0,
+                                   batch.seg_slot, batch.seg_start, max_qlen=batch.max_qlen, min_qlen=batch.min_qlen,
+                                   max_kv_len=batch.max_position + 1, num_q_heads=num_q_heads,
+                                   num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=cache.page_size,
+                                   scale=scale, window=window, splits=getattr(batch, "kv_splits", None),
+                                   short_segments=getattr(batch, "single_segments", 0) or None,
+                                   plan_token=getattr(batch, "plan_token", 0),
+                                   max_portion_kv_len=getattr(batch, "max_portion_kv", 0) or None,
+                                   blocks=mx.empty_rows(*out.shape, form) if form is not None else None)
+    ops.attn_paged_simt(q, out, cache.k_pages, cache.v_pages, cache.block_table, batch.positions,
+                        batch.slot_of_token, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,
+                        head_dim=head_dim, page_size=cache.page_size, scale=scale, window=window)
+    return out

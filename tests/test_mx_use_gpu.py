@@ -320,3 +320,47 @@ def test_attention_that_leaves_blocks(form, D, nq, nkv, contexts):
 
 def _same_rows(a, b):
     return a[2:5] == b[2:5] and all(torch.equal(p, q) for p, q in zip(plain.unpack(a), plain.unpack(b)))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("nq,nkv,window", [(32, 8, 0), (8, 2, 0), (4, 4, 40), (12, 4, 0)])
+@pytest.mark.parametrize("portions", [[(0, 300)], [(0, 2048)], [(700, 64), (0, 33), (5, 500)], [(0, 20), (100, 1)]])
+def test_portions_that_leave_blocks(form, nq, nkv, window, portions):
+    """Prompt portions (position, tokens) whose results leave in blocks, bit for bit those that quantize makes of the same step's; where the step
+    holds decoded tokens too, or rows have padding, the results come as they are."""
+    from arle_amd.kernels import ops
+
+    P, D, T = 16, 128, sum(n for _, n in portions)
+    pages = [(at + n + P - 1) // P for at, n in portions]
+    order = torch.randperm(sum(pages), generator=_g(1)).to(torch.int32)
+    table = torch.zeros(len(portions), max(pages), dtype=torch.int32)
+    for i, part in enumerate(order.split(pages)):
+        table[i, :len(part)] = part
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    k, v = (torch.randn(sum(pages), nkv, *shape, generator=_g(2)).bfloat16().to(DEV) for shape in ((P, D), (D, P)))
+    q = torch.randn(T, nq * D, generator=_g(3)).bfloat16().to(DEV)
+    row0 = [0]
+    for _, n in portions:
+        row0.append(row0[-1] + n)
+    lengths = [n for _, n in portions]
+
+    def run(**kw):
+        out = torch.zeros(T, nq * D, dtype=torch.bfloat16, device=DEV)
+        return ops.attn_paged_mfma(q, out, k, v, table.to(DEV), i32(row0), i32(list(range(len(portions)))), i32([at for at, _ in portions]),
+                                   max_qlen=max(lengths), min_qlen=min(lengths), max_kv_len=max(at + n for at, n in portions), num_q_heads=nq,
+                                   num_kv_heads=nkv, head_dim=D, page_size=P, scale=D**-0.5, window=window, **kw)
+
+    for kw in (dict(portion_splits=1), dict(), dict(portion_splits=2)):
+        want = mx.quantize(run(**kw), form)
+        blocks = mx.empty_rows(T, nq * D, form)
+        blocks.elements.view(torch.uint8).fill_(0x77)
+        blocks.scales.view(torch.uint8).fill_(0x77)
+        got = run(blocks=blocks, **kw)
+        whole = kw == dict(portion_splits=1) and min(lengths) * nq // nkv > 16 and nq * D % 512 == 0
+        assert (got is blocks) or not whole
+        if got is not blocks:
+            assert kw == dict(portion_splits=2) or kw == dict() or not whole
+            got = mx.quantize(got, form)
+        assert _same_rows(got, want), kw
+    with pytest.raises(ops.ShapeError):
+        run(blocks=mx.empty_rows(T + 1, nq * D, form))
