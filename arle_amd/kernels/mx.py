@@ -374,12 +374,14 @@ def _choose(M: int, n_tiles: int, k_tiles: int, bits: int, gated: bool, whole: b
     N = 16 * n_tiles
     if M <= 16 and not gated:
         # us at 8 rows, pairs of columns tiles in 4 waves and K in as many parts as stand / the same whole / single tiles in 8 waves, whole:
-        # 2,560 x 4,096  4.1 (8) / 5.7 / 5.0;  2,560 x 9,728  5.7 (8) / 9.6 / 7.7;  6,144 x 2,560  4.6 (4) / 4.7 / 5.4;
-        # 10,240 x 5,120  8.6 (2) / 10.4 / 10.3
+        # 2,560 x 4,096  4.1 (8) / 5.7 / 5.0;  2,560 x 9,728  5.4 (8) / 9.6 / 7.7;  6,144 x 2,560  4.3 (4) / 4.7 / 5.4;
+        # 10,240 x 5,120  8.6 (2) / 10.4 / 10.3.  Who reads the parts pays for each of them, so that with a norm behind it 1, 2, 4 and 8 parts take
+        # 8.9, 8.1, 8.5 and 9.4 (2,560 x 4,096), 12.8, 10.3, 10.4 and 11.0 (2,560 x 9,728), and a decode step of 8 requests at the Qwen3-4B
+        # widths 2.17, 2.12, 2.11, 2.07 and 2.08 ms with 640, 400, 320, 240 and 160 pairs and parts in all
         pairs = -(-n_tiles // 2)
         if whole:
             return (0 if pairs >= 192 else 1), 1
-        return 0, _even(min(max(1, round(640 / pairs)), 8, max(1, k_tiles // 4)), k_tiles)
+        return 0, _even(min(max(1, round(240 / pairs)), 8, max(1, k_tiles // 4)), k_tiles)
     if M <= 16 and n_tiles <= 1024:
         # us, the few rows' kernel / tiles of 64 x 128, of which there are too few to fill the chip then: 8 x 1,024 x 4,096 6.6 / 10.6, 8 x 3,200 x 1,024 3.7 /
         # 5.4, 16 x 6,144 x 2,048 6.1 / 8.0 (ff x K); 8 x 9,728 x 2,560 9.2 / 9.3, 16 rows 10.0 / 9.3, 8 x 12,288 x 4,096 13.5 / 12.7
