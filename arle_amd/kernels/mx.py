@@ -85,13 +85,20 @@ def padded_width(width: int) -> int:
 _Rows = collections.namedtuple("_Rows", "elements scales width form rows padded bits device")
 
 
+def _checked_fields(cls, fields: tuple, given: int, derived: tuple):
+    if derived and derived != fields[given:]:
+        raise ShapeError(f"{cls.__name__} of {fields[given:]} cannot be {derived}")
+    return tuple.__new__(cls, fields)
+
+
 class MXRows(_Rows):
     """Rows in blocks, MXRows(elements, scales, width, form).  elements: float8_e4m3fn [T, padded] (mxfp8) or uint8 [T, padded / 2] (mxfp4, the number
     with the lower index in the lower half of a byte); scales float8_e8m0fnu [T, padded / 32]; zeros (codes of 0) from `width` to `padded`, the next
     multiple of 512.  Views whose rows lie apart are fine where rows start at multiples of 16 bytes."""
     __slots__ = ()
 
-    def __new__(cls, elements: torch.Tensor, scales: torch.Tensor, width: int, form: str):
+    def __new__(cls, elements: torch.Tensor, scales: torch.Tensor, width: int, form: str, *derived):
+        """derived: the other fields, if given (a tuple put together again from its fields): they have to be what the first four say."""
         bits = _bits(form)
         device = _here(elements, scales)
         if not 1 <= width <= MAX_K:
@@ -105,10 +112,15 @@ class MXRows(_Rows):
         if (e.stride(1) != 1 or s.stride(1) != 1 or e.data_ptr() % 16 or s.data_ptr() % 16
                 or (e.shape[0] > 1 and (e.stride(0) % 16 or s.stride(0) % 16 or max(e.stride(0), s.stride(0)) > 2 * MAX_K))):
             raise ShapeError(f"rows of elements and scales must lie together and start at multiples of 16 bytes, up to {2 * MAX_K} apart")
-        return tuple.__new__(cls, (e, s, int(width), form, e.shape[0], padded, bits, device))
+        return _checked_fields(cls, (e, s, int(width), form, e.shape[0], padded, bits, device), 4, derived)
 
     def __getnewargs__(self):      # of a copy: what it is made from, which is checked again
         return self[:4]
+
+    @classmethod
+    def _make(cls, fields):
+        """What `_replace` makes too: a plain tuple of the fields, which no kernel takes, as nothing has checked them."""
+        return _Rows._make(fields)
 
     def part(self, start: int, stop: int) -> "MXRows":
         """Rows start .. stop - 1, a view."""
@@ -272,7 +284,7 @@ class MXWeight(_Weight):
     the up's, held in turns of 16 with both halves padded with zeros to a multiple of 512."""
     __slots__ = ()
 
-    def __new__(cls, tiles: torch.Tensor, scales: torch.Tensor, n: int, k: int, gated: bool = False):
+    def __new__(cls, tiles: torch.Tensor, scales: torch.Tensor, n: int, k: int, gated: bool = False, *derived):
         device = _here(tiles, scales)
         if n < 1 or k < 1 or (gated and n % 2):
             raise ShapeError(f"a weight of {n} rows of {k} ({'gated' if gated else 'plain'})")
@@ -287,10 +299,14 @@ class MXWeight(_Weight):
         if (tiles.stride() != (1024 * pitch, 1024, 16, 1) or scales.stride()[1:] != (256, 4, 1) or (k_tiles > 4 and scales.stride(0) != 256 * pitch)
                 or pitch < n_tiles or pitch * k_tiles * 2048 > MAX_WEIGHT or tiles.data_ptr() % 16 or scales.data_ptr() % 16):
             raise ShapeError("a step's tiles and scales must lie together, start at multiples of 16 bytes and be equally many apart")
-        return tuple.__new__(cls, (tiles, scales, int(n), int(k), bool(gated), n_tiles, k_tiles, device, pitch))
+        return _checked_fields(cls, (tiles, scales, int(n), int(k), bool(gated), n_tiles, k_tiles, device, pitch), 5, derived)
 
     def __getnewargs__(self):
         return self[:5]
+
+    @classmethod
+    def _make(cls, fields):      # as for rows: nothing that a kernel takes
+        return _Weight._make(fields)
 
     def first(self, rows: int) -> "MXWeight":
         """The weight's first `rows` rows, a multiple of 16: a view."""

@@ -561,8 +561,14 @@ def attn_paged_mfma(q, out, k_pages, v_pages, block_table, seg_row0, seg_slot, s
 
 
 def _need_blocks(blocks, rows: int, width: int, like) -> None:
-    _need(hasattr(blocks, "padded") and (blocks.rows, blocks.width) == (rows, width) and blocks.elements.is_contiguous()
-          and blocks.scales.is_contiguous() and blocks.device == like.get_device(), "blocks must be contiguous mx.MXRows [T, nq*D] on the same device")
+    """What a kernel is to fill is measured here, at its tensors: the fields of a tuple may have been exchanged (`_replace`)."""
+    padded = -(-width // 512) * 512
+    _need(hasattr(blocks, "padded") and (blocks.rows, blocks.width, blocks.padded) == (rows, width, padded)
+          and (blocks.form, blocks.bits) in (("mxfp8", 8), ("mxfp4", 4)) and tuple(blocks.elements.shape) == (rows, padded * blocks.bits // 8)
+          and tuple(blocks.scales.shape) == (rows, padded // 32) and blocks.elements.element_size() == blocks.scales.element_size() == 1
+          and blocks.elements.is_contiguous() and blocks.scales.is_contiguous() and blocks.elements.data_ptr() % 16 == blocks.scales.data_ptr() % 16 == 0
+          and blocks.device == blocks.elements.get_device() == blocks.scales.get_device() == like.get_device(),
+          "blocks must be contiguous mx.MXRows [T, nq*D] on the same device")
 
 
 _PREP_HEAD_DIMS = (64, 128)
