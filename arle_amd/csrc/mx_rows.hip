@@ -102,9 +102,9 @@ __device__ __forceinline__ float4 mx_ld4(const T* p, int col, int width) {   // 
     const float4 v = ld4<T>(p + min(col, width - 4));
     return col < width ? v : float4{0.f, 0.f, 0.f, 0.f};
   } else {
-    const int last = width - 1;
-    const float a = to_float(p[min(col, last)]), b = to_float(p[min(col + 1, last)]), c = to_float(p[min(col + 2, last)]),
-                d = to_float(p[min(col + 3, last)]);
+    const uint32_t at = col, last = width - 1;      // (offsets that are known to be no less than zero take a register each, others two)
+    const float a = to_float(p[min(at, last)]), b = to_float(p[min(at + 1, last)]), c = to_float(p[min(at + 2, last)]),
+                d = to_float(p[min(at + 3, last)]);
     return float4{col < width ? a : 0.f, col + 1 < width ? b : 0.f, col + 2 < width ? c : 0.f, col + 3 < width ? d : 0.f};
   }
 }
@@ -120,18 +120,21 @@ __global__ __launch_bounds__(THREADS) void mx_norm_kernel(float* __restrict__ re
   const int64_t src = rows ? rows[r] : r;
   float* res = residual + src * width;
   const TD* d = delta + src * width;
+  // Up to two groups a thread the weight is on its way beside the row, and as many parts as there is room for.  Four groups of sixteen waves, which
+  // have 128 registers, hold the row, its sum and one part more; the weight, which other rows have left in the caches, comes behind the sum.
+  constexpr bool kWeightFirst = VPT < 4;
   float4 v[VPT], wv[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int col = 4 * (threadIdx.x + j * THREADS);
     v[j] = mx_ld4<float, ALIGNED>(res, col, width);
-    wv[j] = mx_ld4<TW, ALIGNED>(w, col, width);
+    if constexpr (kWeightFirst) wv[j] = mx_ld4<TW, ALIGNED>(w, col, width);
   }
   if (n_delta > 0) {
     float4 sum[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) sum[j] = mx_ld4<TD, ALIGNED>(d, 4 * (threadIdx.x + j * THREADS), width);
-    constexpr int kAhead = VPT == 1 ? 7 : 3;      // parts on their way; past the last one nothing is fetched
+    constexpr int kAhead = VPT == 1 ? 7 : VPT == 2 ? 3 : 1;      // parts on their way; past the last one nothing is fetched
     for (int p = 1; p < n_delta; p += kAhead) {
       float4 e[kAhead][VPT];
 #pragma unroll
@@ -177,6 +180,7 @@ __global__ __launch_bounds__(THREADS) void mx_norm_kernel(float* __restrict__ re
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int col = 4 * (threadIdx.x + j * THREADS);
+    if constexpr (!kWeightFirst) wv[j] = mx_ld4<TW, ALIGNED>(w, col, width);
     const float4 y = {v[j].x * inv * wv[j].x, v[j].y * inv * wv[j].y, v[j].z * inv * wv[j].z, v[j].w * inv * wv[j].w};
     // (a NaN factor on a column past the width would make its zero a NaN)
     const float4 z = {col < width ? y.x : 0.f, col + 1 < width ? y.y : 0.f, col + 2 < width ? y.z : 0.f, col + 3 < width ? y.w : 0.f};
@@ -196,7 +200,9 @@ int mx_norm_launch(float* residual, const void* delta, int n_delta, int64_t delt
       residual, static_cast<const TD*>(delta), n_delta, delta_stride, static_cast<const TW*>(w), elements, scales, rows, width, padded, eps)
   // few rows: a group of columns a thread, so that a row's loads are one trip; many, which hide each other's trips: fewer waves that wait for each
   // other's sums (us, one group a thread / two: 1,024 x 2,560 8.4 / 7.8, 2,048 x 2,560 13.5 / 12.8, 4,096 x 4,096 37.3 / 35.0, 600 x 4,096 8.3 /
-  // 7.8; level at 512 rows, and at 2,048 x 5,120 with four groups instead of two 26.1 / 26.8)
+  // 7.8; level at 512 rows, and at 2,048 x 5,120 with four groups instead of two 26.1 / 26.8).  Past 8,192 columns four groups a thread: 2,048 x 12,288
+  // 42.7 us, 6.5 TB/s (52.3 where three parts ahead and the weight beside the row spill registers), 2,048 x 12,290, whose columns are loaded one by one,
+  // 76, one row of 12,288 with four parts 6.2
   const bool many = n_rows > 512;
   if (padded <= 1024)
     ARLE_MX_NORM(256, 1);
