@@ -318,6 +318,19 @@ static AttnArgs make_args(const void* q, long long q_stride, void* out, long lon
   return a;
 }
 
+// Whether prompt portions run attn_prefill_dma_kernel, and whether their results may leave in blocks (arle_attn_paged_mfma_blocks): portions only, whole keys, rows
+// of whole 512 columns.
+static bool portions_dma(int nkv, int D, int page_size) {
+  return D == 128 && page_size % 8 == 0 && static_cast<long long>(nkv) * page_size * D < (1LL << 31) && g_prefill_dma != 0;
+}
+static bool leaves_blocks(int min_qlen, int nq, int nkv, int D, int page_size, int portion_splits) {
+  return portions_dma(nkv, D, page_size) && nkv > 0 && static_cast<long long>(min_qlen) * (nq / nkv) > 16 && portion_splits == 1 &&
+         static_cast<long long>(nq) * D % 512 == 0;
+}
+extern "C" int arle_attn_leaves_blocks(int min_qlen, int nq, int nkv, int D, int page_size, int portion_splits) {
+  return leaves_blocks(min_qlen, nq, nkv, D, page_size, portion_splits);
+}
+
 // q, out: bfloat16 [token rows, nq*D] (row strides in elements).  Segments describe the packed
 // step: seg_row0[s]..seg_row0[s+1] are the token rows of segment s, whose first token sits at
 // position seg_start[s] of the request in block-table row seg_slot[s]; the cache already holds
@@ -368,9 +381,9 @@ static int paged_mfma(const void* q, long long q_stride, void* out, long long o_
     // prompt portions through the LDS kernel; segments of at most 16 rows (decoded tokens of a mixed
     // step) through the streaming kernel
     dim3 grid((max_rows + kPfRows - 1) / kPfRows, nkv, segments);
-    const bool dma = D == 128 && page_size % 8 == 0 && static_cast<long long>(nkv) * page_size * D < (1LL << 31) && g_prefill_dma != 0;
+    const bool dma = portions_dma(nkv, D, page_size);
     if (blocks != nullptr) {
-      if (!dma || min_rows <= 16 || portion_splits != 1) return static_cast<int>(hipErrorInvalidValue);
+      if (!leaves_blocks(min_qlen, nq, nkv, D, page_size, portion_splits)) return static_cast<int>(hipErrorInvalidValue);
       a.blocks = blocks->elements;
       a.block_scales = blocks->scales;
       a.block_bits = blocks->bits;
@@ -475,7 +488,7 @@ extern "C" int arle_attn_paged_mfma_blocks(const void* q, long long q_stride, vo
                                            float* pws_ml, long long plan_token, const float* sink, float out_scale,
                                            int short_segments, void* elements, void* scales, int bits,
                                            void* stream) {
-  if ((bits != kMx8 && bits != kMx4) || elements == nullptr || scales == nullptr || nq * D % 512 != 0) return static_cast<int>(hipErrorInvalidValue);
+  if ((bits != kMx8 && bits != kMx4) || elements == nullptr || scales == nullptr) return static_cast<int>(hipErrorInvalidValue);
   const MergeBlocks blocks = {static_cast<uint8_t*>(elements), static_cast<uint8_t*>(scales), bits, nq * D};
   return paged_mfma(q, q_stride, out, o_stride, k_pages, v_pages, block_table, table_stride, seg_row0, seg_slot, seg_start, segments,
                     max_qlen, min_qlen, max_kv_len, token_rows, nq, nkv, D, page_size, scale, window, splits, ws_o, ws_ml, portion_splits,

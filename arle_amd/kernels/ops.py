@@ -547,8 +547,7 @@ def attn_paged_mfma(q, out, k_pages, v_pages, block_table, seg_row0, seg_slot, s
     name, more = "arle_attn_paged_mfma", ()
     if blocks is not None:
         _need_blocks(blocks, tokens, num_q_heads * head_dim, q)
-        if (head_dim == 128 and min_qlen * group > _ATTN_ROW_TILE and portion_splits == 1 and page_size % 8 == 0
-                and num_kv_heads * page_size * head_dim < 2**31 and blocks.padded == blocks.width):
+        if lib.function("arle_attn_leaves_blocks")(int(min_qlen), num_q_heads, num_kv_heads, head_dim, page_size, int(portion_splits)):
             name, more = "arle_attn_paged_mfma_blocks", (blocks.elements.data_ptr(), blocks.scales.data_ptr(), blocks.bits)
     lib.call(name, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0),
              k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), block_table.shape[1],
