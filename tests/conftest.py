@@ -22,6 +22,17 @@ def pytest_collection_modifyitems(config, items):
             item.add_marker(skip)
 
 
+@pytest.fixture(autouse=True)
+def product_table_as_it_was():
+    """The table of measured products is the process's: what a test tunes or loads does not choose the kernels of the tests behind it."""
+    ops = sys.modules.get("arle_amd.kernels.ops")
+    before = dict(ops._PRODUCT_TABLE) if ops is not None else None
+    yield
+    if before is not None and ops._PRODUCT_TABLE != before:
+        ops.clear_product_table()
+        ops._PRODUCT_TABLE.update(before)
+
+
 def pytest_sessionfinish(session, exitstatus):
     """With ARLE_TEST_STATS=<file>: the worst maximum and rms errors that the comparisons with the plain
     implementation saw, one line a comparison (what the tolerances are set against)."""
