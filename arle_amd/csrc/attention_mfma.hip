@@ -38,6 +38,7 @@
 
 #include <cstdio>
 #include <mutex>
+#include <type_traits>
 
 namespace arle {
 
@@ -131,13 +132,13 @@ int launch_prefill_lds(const AttnArgs& a, dim3 grid, int min_rows, int max_kv_le
 
 static int g_prefill_groups = -1;  // -1: the launcher decides; 1, 2: forced (measurements and tests)
 
-template <int GROUPS, bool BESIDE = false>
+template <int GROUPS, bool BESIDE = false, int BLOCK_BITS = 0>
 int launch_prefill_dma_groups(const AttnArgs& a, dim3 grid, int min_rows, int cus, int max_kv_len, hipStream_t s, int longs,
                               int beside_parts = 1) {
   const size_t lds = GROUPS * 2 * kDmStageBytes;
   static OnceADevice asked;
-  if (const int e = ask_lds(asked, lds, {reinterpret_cast<const void*>(&attn_prefill_dma_kernel<true, GROUPS, BESIDE>),
-                                         reinterpret_cast<const void*>(&attn_prefill_dma_kernel<false, GROUPS, BESIDE>)}))
+  if (const int e = ask_lds(asked, lds, {reinterpret_cast<const void*>(&attn_prefill_dma_kernel<true, GROUPS, BESIDE, BLOCK_BITS>),
+                                         reinterpret_cast<const void*>(&attn_prefill_dma_kernel<false, GROUPS, BESIDE, BLOCK_BITS>)}))
     return e;
   const long long items = static_cast<long long>(grid.x) * grid.y * longs * a.portion_splits;
   const long long places = (GROUPS == 1 ? 2LL : 1LL) * cus;  // two workgroups of four waves a CU, or one of eight
@@ -158,10 +159,10 @@ int launch_prefill_dma_groups(const AttnArgs& a, dim3 grid, int min_rows, int cu
   // of 64 to 800 tokens behind 0 to 2,300 372 against 387; a fresh prompt of 8,192 tokens 615 against 598.
   const int fixed_rounds = g_prefill_fixed_rounds >= 0 ? g_prefill_fixed_rounds : (max_kv_len <= kDealtMaxKeys ? 1 << 20 : 2);
   if (a.P % kDmKeys == 0)
-    attn_prefill_dma_kernel<true, GROUPS, BESIDE><<<workgroups + beside, GROUPS * kDmWaves * kWave, lds, s>>>(
+    attn_prefill_dma_kernel<true, GROUPS, BESIDE, BLOCK_BITS><<<workgroups + beside, GROUPS * kDmWaves * kWave, lds, s>>>(
         a, min_rows, static_cast<int>(grid.x), static_cast<int>(grid.z), listed, pair_up, fixed_rounds, beside, beside_first, beside_parts);
   else
-    attn_prefill_dma_kernel<false, GROUPS, BESIDE><<<workgroups + beside, GROUPS * kDmWaves * kWave, lds, s>>>(
+    attn_prefill_dma_kernel<false, GROUPS, BESIDE, BLOCK_BITS><<<workgroups + beside, GROUPS * kDmWaves * kWave, lds, s>>>(
         a, min_rows, static_cast<int>(grid.x), static_cast<int>(grid.z), listed, pair_up, fixed_rounds, beside, beside_first, beside_parts);
   if (a.portion_splits > 1) launch_merge_portions(a, grid, cus, s);
   return launch_status();
@@ -189,8 +190,13 @@ int launch_prefill_dma(const AttnArgs& a, dim3 grid, int min_rows, int max_qlen,
   const bool two = g_prefill_groups >= 0 ? g_prefill_groups == 2
                                          : (4 * items > cus && (2 * items <= 3LL * cus || (unequal && items <= 2LL * cus)));
   const int longs = static_cast<int>(grid.z);
-  return two ? launch_prefill_dma_groups<2>(a, grid, min_rows, cus, max_kv_len, s, longs)
-             : launch_prefill_dma_groups<1>(a, grid, min_rows, cus, max_kv_len, s, longs);
+  const auto go = [&](auto bits) {
+    constexpr int kBits = decltype(bits)::value;
+    return two ? launch_prefill_dma_groups<2, false, kBits>(a, grid, min_rows, cus, max_kv_len, s, longs)
+               : launch_prefill_dma_groups<1, false, kBits>(a, grid, min_rows, cus, max_kv_len, s, longs);
+  };
+  if (a.blocks == nullptr) return go(std::integral_constant<int, 0>{});
+  return a.block_bits == kMx8 ? go(std::integral_constant<int, kMx8>{}) : go(std::integral_constant<int, kMx4>{});
 }
 
 // Portions and, in the same launch, the step's short segments: `parts` workgroups of four waves for each of them and kv

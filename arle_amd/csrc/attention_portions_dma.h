@@ -50,11 +50,14 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // One launch takes the place of two on streams of their own that were forked and joined around them, and spares a merge
 // where a segment's keys are not cut (32 requests at 1,024 tokens beside a portion of 512 behind 0, 512, 1,024 and
 // 1,536 at 32 q heads over 8 kv heads, us a layer: 59, 60, 63, 73 -> 36, 43, 45, 55).
-template <bool WHOLE, int GROUPS, bool BESIDE>
+//
+// BLOCK_BITS: 0, or results leave in blocks of 32 with elements of so many bits (attention_blocks.h; whole keys only).
+template <bool WHOLE, int GROUPS, bool BESIDE, int BLOCK_BITS = 0>
 __global__ __launch_bounds__(GROUPS* kDmWaves* kWave, GROUPS == 1 ? 2 : 1) void attn_prefill_dma_kernel(
     const AttnArgs a, int min_rows, int blocks_x, int segments, int listed, int pair_up, int fixed_rounds, int beside,
     int beside_first, int beside_parts) {
   static_assert(!BESIDE || GROUPS == 1, "a workgroup of decoded tokens is four waves");
+  static_assert(!BESIDE || BLOCK_BITS == 0, "decoded tokens' results are rows");
   constexpr int D = kDmD;
   extern __shared__ __align__(16) unsigned char lds_all[];
   __shared__ unsigned int item_of_workgroup;
@@ -468,7 +471,7 @@ __global__ __launch_bounds__(GROUPS* kDmWaves* kWave, GROUPS == 1 ? 2 : 1) void 
 
   // o[dt][r] is O^T[d = 32 dt + 8 (r / 4) + 4 h + r % 4][this lane's row]
   if (row_ok) {
-    if (parts > 1) {
+    if (BLOCK_BITS == 0 && parts > 1) {
       const int64_t slot = ((static_cast<int64_t>(row0 + my_tok) * a.nq + my_head) * parts + part);
       float* wo = a.pws_o + slot * D;
 #pragma unroll
@@ -483,22 +486,27 @@ __global__ __launch_bounds__(GROUPS* kDmWaves* kWave, GROUPS == 1 ? 2 : 1) void 
       }
     } else {
       const float inv_l = row_factor(a.sink, a.out_scale, my_head, m, l);
-      uint16_t* op = a.out + static_cast<int64_t>(row0 + my_tok) * a.o_stride + my_head * D;
+      if constexpr (BLOCK_BITS == 0) {
+        uint16_t* op = a.out + static_cast<int64_t>(row0 + my_tok) * a.o_stride + my_head * D;
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        uint2 w[4];
+        for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          w[q].x = pack_bf16x2(o[dt][4 * q] * inv_l, o[dt][4 * q + 1] * inv_l);
-          w[q].y = pack_bf16x2(o[dt][4 * q + 2] * inv_l, o[dt][4 * q + 3] * inv_l);
-        }
-        if (a.blocks == nullptr) {
+          for (int q = 0; q < 4; ++q) {
+            uint2 w;
+            w.x = pack_bf16x2(o[dt][4 * q] * inv_l, o[dt][4 * q + 1] * inv_l);
+            w.y = pack_bf16x2(o[dt][4 * q + 2] * inv_l, o[dt][4 * q + 3] * inv_l);
+            *reinterpret_cast<uint2*>(op + 32 * dt + 8 * q + 4 * h) = w;
+          }
+      } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) *reinterpret_cast<uint2*>(op + 32 * dt + 8 * q + 4 * h) = w[q];
-        } else if (a.block_bits == kMx8) {
-          leave_block<kMx8>(a, row0 + my_tok, my_head * D + 32 * dt, h, w);
-        } else {
-          leave_block<kMx4>(a, row0 + my_tok, my_head * D + 32 * dt, h, w);
+        for (int dt = 0; dt < D / 32; ++dt) {
+          uint2 w[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            w[q].x = pack_bf16x2(o[dt][4 * q] * inv_l, o[dt][4 * q + 1] * inv_l);
+            w[q].y = pack_bf16x2(o[dt][4 * q + 2] * inv_l, o[dt][4 * q + 3] * inv_l);
+          }
+          leave_block<BLOCK_BITS>(a, row0 + my_tok, my_head * D + 32 * dt, h, w);
         }
       }
     }
