@@ -431,7 +431,7 @@ def _per_split(M: int, k_tiles: int, bits: int, variant: int, splits: int) -> in
     steps = k_tiles if few else k_tiles // 4
     if splits == 1:
         return steps
-    per_split = -(-steps // splits)
+    per_split = -(-steps // splits) if splits > 0 else 0
     if splits < 1 or splits > 65535 or (splits - 1) * per_split >= steps:
         raise ShapeError(f"{splits} parts of {steps} steps: some would have none")
     return per_split
@@ -455,7 +455,7 @@ def _checked(x: MXRows, w: MXWeight, gated: bool) -> int:
 def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partials_ok: bool = False, *, variant: int | None = None,
          splits: int | None = None) -> torch.Tensor:
     """x [T, K] . w [N, K]^T with sums of 32 bits -> [T, N] in `out_dtype`; with `partials_ok` possibly a float32 stack [S, T, N] whose
-    sum over S, in order, is the product (as Linear's)."""
+    sum over S, in order, is the product (as Linear's).  The sizes choose the kernel, or `variant` names it and `splits` its parts of K (default: 1)."""
     device = _checked(x, w, False)
     code = _CODES.get(out_dtype)
     if code is None:
@@ -466,9 +466,11 @@ def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partia
     if M == 0:
         return _empty(0, N, dtype=out_dtype, device=on)
     if variant is None:
+        if splits is not None:
+            raise ShapeError(f"{splits} parts of K without the variant that walks them: the sizes choose both, or the caller does")
         variant, splits, per_split = _plan(M, n_tiles, k_tiles, bits, False, not partials_ok)
     else:
-        splits = splits or 1
+        splits = 1 if splits is None else splits
         if variant == GATED_ROWS:
             raise ShapeError(f"variant {variant} makes blocks")
         per_split = _per_split(M, k_tiles, bits, variant, splits)

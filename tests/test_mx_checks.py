@@ -51,3 +51,13 @@ def test_blocks_are_measured_before_a_kernel_fills_them(no_gpu):
                     rows[:3], None):
             with pytest.raises(ops.ShapeError):
                 ops._need_blocks(bad, 3, 600, like)
+
+
+def test_parts_of_k_go_with_a_variant(no_gpu):
+    """A number of parts that nothing would follow is refused, and so is none."""
+    x, w = _rows(3, 1200)[2], mx.lay_weight(_rows(40, 1200, "mxfp4")[2])
+    for args in (dict(splits=2), dict(splits=1), dict(splits=4, partials_ok=True), dict(variant=3, splits=0), dict(variant=0, splits=0), dict(variant=0, splits=-1)):
+        with pytest.raises(ops.ShapeError):
+            mx.gemm(x, w, **args)
+    with pytest.raises(AssertionError, match="launched"):
+        mx.gemm(x, w, variant=3, splits=3)
