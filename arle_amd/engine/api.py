@@ -17,7 +17,7 @@ import os
 from dataclasses import dataclass, field
 
 from ..sampling import Sampler, SamplingParams
-from .engine import Engine
+from .engine import Engine, EngineError, ROW_FORM
 from .scheduler import STOP, Scheduler, SchedulerConfig
 
 
@@ -87,7 +87,7 @@ class LLM:
                  max_prefill_tokens: int | None = None, prefill_max_requests: int | None = None, seed: int = 42,
                  cuda_graph: bool = True, weight_tiles: bool | None = None, mem_fraction_static: float = 0.85,
                  async_overlap: bool = True, warm_up: bool = False, tune_products: bool | str = False,
-                 weight_form: str | None = None, row_form: str = "mxfp8"):
+                 weight_form: str | None = None, row_form: str = ROW_FORM):
         """model: a model folder, or an Engine that is already built.
 
         kv_cache_tokens: tokens the paged cache holds over all live requests.  Default: sized from the GPU's
@@ -102,7 +102,8 @@ class LLM:
         num_slots: requests that run at a time; None: as many requests of max_seq_len tokens as the cache holds, from 4
         to 128 (the reference's --num-slots left unset).
         cuda_graph, weight_tiles: as for Engine (captured steps; the decode-friendly second copy of the weights).
-        weight_form, row_form: as for Engine (projections held in 4 bits, the rows that meet them in 8 or 4).
+        weight_form, row_form: as for Engine (projections held in 4 bits, the rows that meet them in 8 or 4); of an Engine that is built
+        already, what it was built with or nothing.
         async_overlap: decode steps are launched from the last step's tokens on the GPU, and those are read back
         while the new step runs (SchedulerConfig.async_overlap); the tokens are the same either way.
         tune_products: measure which kernel runs each of this model's matrix products fastest at each row count and
@@ -113,6 +114,9 @@ class LLM:
         reference's scheduler does when it starts; otherwise each is captured at its first step.
         """
         if isinstance(model, Engine):
+            if (weight_form is not None or row_form != ROW_FORM) and (weight_form, row_form) != (model.rt.weight_form, model.rt.row_form):
+                raise EngineError(f"the engine was built with weight_form {model.rt.weight_form!r} and row_form {model.rt.row_form!r}; "
+                                  f"it cannot be given {weight_form!r} and {row_form!r} now")
             self.engine = model
         else:
             from ..config.registry import load_model_config

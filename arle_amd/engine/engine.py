@@ -61,13 +61,16 @@ def parse_dtype(name) -> torch.dtype:
         raise EngineError(f"unknown dtype {name!r}; use bfloat16 or float32") from None
 
 
+ROW_FORM = "mxfp8"      # of the rows that meet weights held in 4 bits, if the caller names none
+
+
 class Engine:
     def __init__(self, spec, tensors: dict, *, dtype=torch.bfloat16, device=None,
                  page_size: int = DEFAULT_PAGE_SIZE, max_tokens: int | None = None,
                  num_pages: int | None = None, max_slots: int | None = 4,
                  max_request_tokens: int | None = None, cuda_graph: bool = True,
                  weight_tiles: bool | None = None, mem_fraction_static: float = DEFAULT_MEM_FRACTION_STATIC,
-                 product_table=None, weight_form: str | None = None, row_form: str = "mxfp8",
+                 product_table=None, weight_form: str | None = None, row_form: str = ROW_FORM,
                  _owns_tensors: bool = False):
         """
         max_tokens: tokens the cache holds over all live requests (num_pages = ceil(max_tokens / page_size)
@@ -89,7 +92,7 @@ class Engine:
             the input with a power of two each (4.25 bits a weight), made from the checkpoint's weights when the engine is built;
             norms, embedding, head, cache and attention stay as they are.  The rows that meet them are made into blocks by the kernel in front
             (norm, activation, attention) as `row_form` says: "mxfp8" (e4m3) or "mxfp4".  For designs whose mixers and feed-forwards have
-            that form (the Qwen3 dense decoder), in bfloat16.  None: as the checkpoint holds them.
+            that form (the Qwen3 dense decoder), in bfloat16.  None: as the checkpoint holds them, and no row_form of its own.
         weight_tiles: hold every bfloat16 projection weight a second time in the layout that the few-rows
             kernels stream fastest (decode steps about a tenth faster, twice the weight memory), and the projections
             that a norm and another projection stand behind (o and down, the last down not) a third time where they have 769 to
@@ -102,8 +105,7 @@ class Engine:
         self.spec = spec
         if product_table is not None:
             ops.load_product_table(product_table)
-        if weight_form is not None:
-            self._check_weight_form(spec, weight_form, row_form)
+        self._check_weight_form(spec, weight_form, row_form)
         if weight_tiles is None:
             held = sum(t.numel() * t.element_size() for t in tensors.values() if t.dim() == 2)
             weight_tiles = 2 * held * 3 <= torch.cuda.get_device_properties(self.device).total_memory
@@ -158,11 +160,15 @@ class Engine:
         self.graph_replays = 0
         self._warm_total = None       # the contexts' total that a step of `warm_up` stands for
 
-    def _check_weight_form(self, spec, weight_form: str, row_form: str) -> None:
-        if weight_form != "mxfp4":
-            raise EngineError(f"unknown weight_form {weight_form!r}; use mxfp4, or None for the checkpoint's own")
+    def _check_weight_form(self, spec, weight_form: str | None, row_form: str) -> None:
         if row_form not in mx.BITS:
             raise EngineError(f"unknown row_form {row_form!r}; use {' or '.join(mx.BITS)}")
+        if weight_form is None:
+            if row_form != ROW_FORM:
+                raise EngineError(f"row_form {row_form!r} is for the rows that meet weights held in a weight_form, and none was given")
+            return
+        if weight_form != "mxfp4":
+            raise EngineError(f"unknown weight_form {weight_form!r}; use mxfp4, or None for the checkpoint's own")
         if self.dtype != torch.bfloat16:
             raise EngineError(f"weight_form {weight_form!r} needs dtype bfloat16")
         for layer in spec.layers:
