@@ -1279,6 +1279,21 @@ def design_bench(args, design: str, models: dict, q: dict, layers: int, design_w
     return 0
 
 
+# modes of the command line that build engines of their own, or sort a step's kernels by the names of those in bfloat16
+OWN_ENGINES = ("ceilings", "tune_products", "sweep", "first_token", "generate", "gaps", "parts_only")
+
+
+def forms_are_heard(ap, args) -> None:
+    """--weight-form and --row-form are the default workload's: elsewhere, or without what they go with, they end the run."""
+    if args.weight_form is None:
+        if args.row_form != "mxfp8":
+            ap.error("--row-form goes with --weight-form")
+        return
+    mode = next((m for m in OWN_ENGINES if getattr(args, m)), None)
+    if mode is not None or args.workload != "qwen3-4b":
+        ap.error(f"--weight-form is for the default workload (and --prefill-only), not for {f'--workload {args.workload}' if mode is None else '--' + mode.replace('_', '-')}")
+
+
 def main() -> int:
     global PAGE, PROMPT
     ap = argparse.ArgumentParser()
@@ -1296,7 +1311,7 @@ def main() -> int:
                          "next step is launched from the tokens on the GPU, as the scheduler does)")
     ap.add_argument("--no-weight-tiles", action="store_true",
                     help="without the second copy of the projection weights that the few-rows kernels stream")
-    ap.add_argument("--weight-form", choices=["mxfp4"], default=None, help="projections of the default workload held in 4 bits")
+    ap.add_argument("--weight-form", choices=["mxfp4"], default=None, help="projections of the default workload held in 4 bits (other modes refuse it)")
     ap.add_argument("--row-form", choices=["mxfp8", "mxfp4"], default="mxfp8", help="the rows that meet them")
     ap.add_argument("--no-parts", action="store_true",
                     help="skip the breakdown of the step's time by part of the model (a profiled step)")
@@ -1328,6 +1343,7 @@ def main() -> int:
                          "the Gufasun design beside Qwen3 at equal widths and depth (--shape, --layers, --batch, --prompt-len)")
     ap.add_argument("--shape", default="4b", choices=["4b", "8b"], help="--workload gufasun / sovutar / tazitar / retudra / nafezen / pozirax: whose widths")
     args = ap.parse_args()
+    forms_are_heard(ap, args)
     if args.gpus != 1:
         print(f"bench.py measures one GPU: this engine has no multi-GPU path (asked for --gpus {args.gpus})")
         return 2
