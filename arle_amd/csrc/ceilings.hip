@@ -1,5 +1,5 @@
-// Two measuring kernels, no part of a model step: what one MI355X gives to a kernel that only reads memory, and
-// to one that only multiplies on the matrix cores.  The benchmark reports the engine's kernels against these
+// Three measuring kernels, no part of a model step: what one MI355X gives to a kernel that only reads memory, and
+// to two that only multiply on the matrix cores.  The benchmark reports the engine's kernels against these
 // figures beside the published peaks (8 TB/s, 2.5 PFLOP/s bfloat16), which no kernel reaches.
 //
 //   arle_ceiling_read:  workgroups that stay (one or two a compute unit) read `bytes` in 16-byte pieces a lane,
@@ -11,6 +11,9 @@
 //                       the chip's clock follows its power, and products of operands whose bits differ draw more
 //                       (with all 256 compute units busy 1.65 GHz instead of 2.2 and more, measured), so the second
 //                       is the ceiling for real data.
+//
+//   arle_ceiling_mfma_scaled:  the same with eight independent v_mfma_scale_f32_32x32x64_f8f6f4, 2 * 32 * 32 * 64 flops each: one operand
+//                       e2m1, the other e4m3 or e2m1 (what products of rows with a weight in 4 bits run on), scales of 1.
 #include "common.h"
 
 namespace arle {
@@ -70,6 +73,34 @@ __global__ __launch_bounds__(256) void ceiling_mfma_kernel(int iters, int random
   if (total == 0.123f) sink[0] = total;
 }
 
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+template <int BITS>
+__global__ __launch_bounds__(256) void ceiling_mfma_scaled_kernel(int iters, int random_operands, float* sink) {
+  const uint32_t seed = 0x3f803f80u + threadIdx.x;
+  // e4m3: a random sign, mantissa and last bit of an exponent around 1.0 a byte, or 1.0; e2m1: any bits, or 1.0 throughout
+  auto bits8 = [&](uint32_t mul) { return static_cast<int>(random_operands ? ((seed * mul) & 0x8f8f8f8fu) | 0x30303030u : 0x38383838u); };
+  auto bits4 = [&](uint32_t mul) { return static_cast<int>(random_operands ? seed * mul : 0x22222222u); };
+  const i32x8 w = {bits4(2654435761u), bits4(40503u), bits4(69069u), bits4(1664525u), 0, 0, 0, 0};
+  i32x8 x = {bits4(22695477u), bits4(134775813u), bits4(1103515245u), bits4(214013u), 0, 0, 0, 0};
+  if constexpr (BITS == 8)
+    x = i32x8{bits8(22695477u), bits8(134775813u), bits8(1103515245u), bits8(214013u), bits8(2246822519u), bits8(3266489917u), bits8(668265263u), bits8(374761393u)};
+  f32x16 acc[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[u][r] = 0.f;
+  for (int it = 0; it < iters; ++it) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      acc[u] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, acc[u], 4, BITS == 8 ? 0 : 4, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+  }
+  float total = 0.f;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) total += acc[u][0] + acc[u][15];
+  if (total == 0.123f) sink[0] = total;
+}
+
 }  // namespace arle
 
 using namespace arle;
@@ -96,5 +127,16 @@ extern "C" int arle_ceiling_mfma(int shape, int iters, int workgroups, int rando
     ceiling_mfma_kernel<32><<<workgroups, 256, 0, s>>>(iters, random_operands, static_cast<float*>(sink));
   else
     ceiling_mfma_kernel<16><<<workgroups, 256, 0, s>>>(iters, random_operands, static_cast<float*>(sink));
+  return launch_status();
+}
+
+// bits of the other operand's elements: 8 (e4m3) or 4 (e2m1).  A wave does iters * 1048576 flops; workgroups of four waves.
+extern "C" int arle_ceiling_mfma_scaled(int bits, int iters, int workgroups, int random_operands, void* sink, void* stream) {
+  if (workgroups < 1 || iters < 1 || (bits != 4 && bits != 8)) return static_cast<int>(hipErrorInvalidValue);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (bits == 8)
+    ceiling_mfma_scaled_kernel<8><<<workgroups, 256, 0, s>>>(iters, random_operands, static_cast<float*>(sink));
+  else
+    ceiling_mfma_scaled_kernel<4><<<workgroups, 256, 0, s>>>(iters, random_operands, static_cast<float*>(sink));
   return launch_status();
 }

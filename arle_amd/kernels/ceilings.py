@@ -45,6 +45,16 @@ def mfma_rate(device="cuda:0", shape: int = 32, iters: int = 20000, repeats: int
     """Flops a second of waves that do nothing but bfloat16 matrix-core products (16 waves a compute unit, or
     `workgroups` of four waves over the chip).  `random_operands`: operands whose bits differ, as real data's do;
     the chip clocks lower under them than under operands that are all alike."""
+    return _rate("arle_ceiling_mfma", shape, 262144.0, device, iters, repeats, random_operands, workgroups)
+
+
+def mfma_scaled_rate(device="cuda:0", form: str = "mxfp8", iters: int = 20000, repeats: int = 3, random_operands: bool = True,
+                     workgroups: int | None = None) -> float:
+    """The same of scaled products of a weight in 4 bits (e2m1) with rows in e4m3 ("mxfp8") or e2m1 ("mxfp4")."""
+    return _rate("arle_ceiling_mfma_scaled", {"mxfp8": 8, "mxfp4": 4}[form], 1048576.0, device, iters, repeats, random_operands, workgroups)
+
+
+def _rate(name: str, kind: int, flops: float, device, iters: int, repeats: int, random_operands: bool, workgroups: int | None) -> float:
     dev = torch.device(device)
     cus = torch.cuda.get_device_properties(dev).multi_processor_count
     sink = torch.zeros(4, dtype=torch.float32, device=dev)
@@ -53,7 +63,7 @@ def mfma_rate(device="cuda:0", shape: int = 32, iters: int = 20000, repeats: int
     for _ in range(repeats + 1):
         torch.cuda.synchronize(dev)
         t = time.perf_counter()
-        lib.call("arle_ceiling_mfma", shape, iters, wgs, 1 if random_operands else 0, sink.data_ptr(), _stream())
+        lib.call(name, kind, iters, wgs, 1 if random_operands else 0, sink.data_ptr(), _stream())
         torch.cuda.synchronize(dev)
         best = min(best, time.perf_counter() - t)
-    return wgs * 4 * iters * 262144.0 / best
+    return wgs * 4 * iters * flops / best

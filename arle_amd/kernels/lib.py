@@ -146,6 +146,7 @@ SIGNATURES = {
     "arle_mx_gemm": ("mx_gemm", [_i, _i, _i, _p, _ll, _p, _ll, _p, _p, _p, _ll, _p, _ll, _i, _i, _i, _i, _i, _i, _i, _p]),
     "arle_ceiling_read": ("ceilings", [_p, _ll, _i, _p, _p, _p]),
     "arle_ceiling_mfma": ("ceilings", [_i, _i, _i, _i, _p, _p]),
+    "arle_ceiling_mfma_scaled": ("ceilings", [_i, _i, _i, _i, _p, _p]),
 }
 
 _libs: dict = {}

@@ -242,6 +242,7 @@ def ceilings() -> int:
     small = c.read_bandwidth(launches=40)
     m32, m16 = c.mfma_rate(shape=32), c.mfma_rate(shape=16)
     same32 = c.mfma_rate(shape=32, random_operands=False)
+    scaled = {form: (c.mfma_scaled_rate(form=form), c.mfma_scaled_rate(form=form, random_operands=False)) for form in ("mxfp8", "mxfp4")}
     cus = torch.cuda.get_device_properties(0).multi_processor_count
     # one workgroup of four waves a busy compute unit: what a product costs in time says what the clock is (32 cycles)
     by_busy = {n: c.mfma_rate(shape=32, workgroups=n, repeats=2) for n in (cus // 8, cus // 2, 3 * cus // 4, cus)}
@@ -253,6 +254,7 @@ def ceilings() -> int:
         "mfma_bf16_32x32x16_tflops": round(m32 / 1e12, 1), "mfma_bf16_16x16x32_tflops": round(m16 / 1e12, 1),
         "mfma_frac_of_peak": round(max(m32, m16) / PEAK_FLOPS["bf16"], 4),
         "mfma_bf16_32x32x16_same_operands_tflops": round(same32 / 1e12, 1),
+        **{f"mfma_scaled_{form}_x_mxfp4{what}_tflops": round(v / 1e12, 1) for form, rates in scaled.items() for what, v in zip(("", "_same_operands"), rates)},
         "mfma_clock_ghz_by_busy_cus": {str(n): round(v / (n * 4 * 32768.0 / 32.0) / 1e9, 2) for n, v in by_busy.items()}}))
     return 0
 
