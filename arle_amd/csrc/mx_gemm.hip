@@ -208,8 +208,8 @@ __global__ __launch_bounds__(WAVES* kWave) void mx_gemm_rows_kernel(const MxArgs
 //     9,728, 43.3 / 44.1.)  The small tiles' eight stages reach further than the next tile, so theirs have one tile each.
 //
 // What bounds it (MI355X): 4,096 x 4,096 x 12,288 in 256 x 256, one workgroup a compute unit, takes 134 us, 3.1 PFLOP/s; the same without its
-// loads 115, with nothing but its loads 81 (14.5 TB/s from the L2s), the matrix cores are busy 87 % of the time and the clock is down to
-// 1.9 GHz.  Shorter ones are bound by what a compute unit does at once: 2,048 x 2,560 x 9,728 in 128 x 192 44 us, 42 with every load a hit in the
+// loads 115, with nothing but its loads 81 (14.5 TB/s from the L2s), the matrix cores are busy 87 % of the time (80 with the activation at K = 4,096, 56 to 62 with
+// X in e2m1, whose products take half as long beside the same reads of W) and the clock is down to 1.9 GHz.  Shorter ones are bound by what a compute unit does at once: 2,048 x 2,560 x 9,728 in 128 x 192 44 us, 42 with every load a hit in the
 // first cache, 38 without loads, 35 without reads of LDS either; 4,096 x 6,144 x 4,096 with X in e2m1 55, 51, 43 and 35.  Waves that only load (one
 // or two a workgroup) cannot send fast enough: 45 -> 55 us.
 template <int BITS, int MT, int TN, int RW, int CW, int STAGES, int WAVES_A_SIMD, int EPI>

@@ -365,6 +365,13 @@ ROW_VARIANTS, GATED_ROWS = (0, 1), 9                                        # of
 #   gate|up, 2,048 x 9,728 x 2,560         143.0     81.4     78.9     85.3
 #   gate|up, 4,096 x 12,288 x 4,096        546.3    325.0    298.1    276.2
 #   the same, 4 bits                                279.4    241.4    197.2
+# (gate|up before the activation's last bits, 1 to 3 % more since).  What the choice comes to, us, with add_rmsnorm behind it that reads the parts of K
+# (variant, parts): chosen / best of all
+#   32 x 4,096 x 12,288   (2, 4) 13.4 / -           64 x 2,560 x 9,728    (3, 7) 14.8 / (2, 4) 14.4     the same, 4 bits       (3, 7) 14.1 / (3, 4) 13.9
+#   128 x 4,096 x 12,288  (3, 4) 18.1 / -           256 x 4,096 x 12,288  (3, 2) 23.8 / -               384 x 4,096 x 12,288   (4, 2) 33.0 / (5, 4) 32.6
+#   512 x 2,560 x 9,728   (7, 4) 27.7 / (3, 1) 26.9 768 x 4,096 x 12,288  (4, 1) 54.5 / (5, 2) 47.7     1,024 x 4,096 x 12,288 (4, 1) 57.4 / 54.7 (itself again)
+#   1,024 x 2,560 x 9,728 (7, 2) 39.2 / -           64 x 5,120 x 25,600   (3, 4) 29.0 / -               512 x 5,120 x 25,600   (7, 2) 75.2 / 72.8 (itself)
+# and gate|up, ff x K of 25,600 x 5,120: 1 row (3) 31.7 / (9) 28.0, 16 rows of 4 bits (5) 35.6 / (9) 31.2, 64 rows (3) 38.3 / (5) 36.8, 512 rows (6) 112 / -.
 _TILES = {2: (32, 64, 2, 1.5, 0.15, 0.36, 0.15, 0.36), 3: (64, 128, 1, 2.5, 0.28, 0.28, 0.25, 0.25), 4: (128, 128, 2, 2.5, 0.43, 0.78, 0.38, 0.68),
           5: (128, 256, 1, 3.0, 0.48, 0.715, 0.30, 0.55), 6: (256, 256, 1, 5.0, 0.95, 1.32, 0.55, 0.92), 7: (128, 192, 1, 3.0, 0.44, 0.59, 0.36, 0.47),
           8: (256, 192, 1, 4.0, 0.80, 1.05, 0.53, 0.73)}
