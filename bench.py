@@ -49,10 +49,13 @@ def layer_params(c) -> int:
     return h * (q + 2 * kv) + q * h + 3 * h * i
 
 
-def decode_bytes(c, batch: int, context: float, elt: int = 2) -> float:
-    """Bytes one decode step has to read: every weight once and the cache of the live requests."""
+MXFP4_BYTES = 17 / 32      # a number in 4 bits and its part of a byte for every 32 of them
+
+
+def decode_bytes(c, batch: int, context: float, elt: int = 2, projections: float | None = None) -> float:
+    """Bytes one decode step has to read: every weight once and the cache of the live requests.  projections: bytes of a projection's number, if other than elt."""
     L, h = c["num_hidden_layers"], c["hidden_size"]
-    weights = (L * (layer_params(c) + 2 * h + 2 * c["head_dim"]) + h + c["vocab_size"] * h) * elt
+    weights = L * layer_params(c) * (elt if projections is None else projections) + (L * (2 * h + 2 * c["head_dim"]) + h + c["vocab_size"] * h) * elt
     kv = batch * context * 2 * L * c["num_key_value_heads"] * c["head_dim"] * elt
     return weights + kv
 
@@ -1520,7 +1523,7 @@ def main() -> int:
     dt, ctx_mean = decode_run(args.batch, args.steps, args.warmup)
     ms_per_step = dt / args.steps * 1e3
     value = args.batch * args.steps / dt
-    achieved = decode_bytes(raw, args.batch, ctx_mean, elt) / (dt / args.steps) / 1e9
+    achieved = decode_bytes(raw, args.batch, ctx_mean, elt, MXFP4_BYTES if args.weight_form else None) / (dt / args.steps) / 1e9
     print(f"[bench] decode b{args.batch}: {value:.1f} tok/s, {ms_per_step:.3f} ms/step", file=sys.stderr, flush=True)
     points = {}
     if not args.no_points:
@@ -1558,7 +1561,6 @@ def main() -> int:
         line["metric"] += held
         line["dtype"] = f"{dkey}, products in {args.row_form} x {args.weight_form}"
         line["config"].update(weight_form=args.weight_form, row_form=args.row_form)
-        line.pop("roofline")      # of the bytes of bfloat16 weights
     if args.batch != 8:
         line["metric"] = line["metric"].replace("batch 8", f"batch {args.batch}")
     print(json.dumps(line))

@@ -29,3 +29,12 @@ def test_rows_go_with_weights(monkeypatch, capsys):
 def test_the_default_workload_takes_them(args, monkeypatch, capsys):
     monkeypatch.setattr(sys, "argv", ["bench.py", "--gpus", "2", *args])      # ends behind the arguments: no engine for two GPUs
     assert bench.main() == 2 and "one GPU" in capsys.readouterr().out
+
+
+def test_a_step_reads_its_projections_in_the_form_that_they_are_held_in():
+    c = bench.QWEN3_4B
+    layers = c["num_hidden_layers"] * bench.layer_params(c)
+    whole, held = bench.decode_bytes(c, 8, 2064.0), bench.decode_bytes(c, 8, 2064.0, 2, bench.MXFP4_BYTES)
+    assert whole == bench.decode_bytes(c, 8, 2064.0, 2, 2) and whole - held == layers * (2 - 17 / 32)
+    # 36 layers of q|k|v, o, gate|up and down: 4.25 bits a number, 1.9 GB of them; embedding and norms stay as they are
+    assert layers * bench.MXFP4_BYTES == 36 * (6144 * 2560 + 2560 * 4096 + 3 * 2560 * 9728) * 17 / 32
