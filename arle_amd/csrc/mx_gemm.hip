@@ -582,7 +582,9 @@ int mx_tiles_launch(MxArgs a, int splits, hipStream_t s) {
   // workgroups that stay: as many as run at once, each going on to its next tile while the results of the one before leave
   const int places = (a.m_blocks * a.n_blocks + 7) / 8 * 8;
   constexpr int kByLds = 160 * 1024 / kLds, kByWaves = 4 * WAVES_A_SIMD / (RW * CW), kHeld = kByLds < kByWaves ? kByLds : kByWaves, kUnits = 256;
-  kernel<<<dim3(STAGES <= 5 && splits == 1 ? min(places, kHeld * kUnits) : places, splits), RW * CW * kWave, kLds, s>>>(a);
+  const int workgroups = STAGES <= 5 && splits == 1 ? min(places, kHeld * kUnits) : places;
+  if (static_cast<long long>(workgroups) * (RW * CW * kWave) >= 1LL << 32) return static_cast<int>(hipErrorInvalidValue);   // 2^36 results and more
+  kernel<<<dim3(workgroups, splits), RW * CW * kWave, kLds, s>>>(a);
   return launch_status();
 }
 

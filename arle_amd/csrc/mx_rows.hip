@@ -12,6 +12,15 @@
 
 namespace arle {
 
+// Rows of one launch: a grid of 2^32 threads or more along an axis is refused, or taken modulo 2^32 without a word.
+constexpr int kMxLaunchRows = 1 << 21;
+template <typename Launch>
+int mx_by_launches(int rows, Launch launch) {      // launch(first row, how many)
+  for (int64_t at = 0; at < rows; at += kMxLaunchRows)
+    if (const int e = launch(at, rows - at < kMxLaunchRows ? static_cast<int>(rows - at) : kMxLaunchRows)) return e;
+  return 0;
+}
+
 // ---- quantisation: a thread owns eight columns of kRows rows, four lanes a block.  Bound by memory: 19,456 x 2,560 of bfloat16 to e2m1 24.3 us, 5.2
 // TB/s, the rate of a copy.  Two rows a thread from 1,025 rows on (us, one / two / four / eight rows: 27.8 / 24.3 / 24.6 / 25.6; 2,048 x 4,096 to e4m3
 // 7.0 / 6.6 / 7.2 / 7.4); with fewer, one, for as many workgroups as there can be.
@@ -194,16 +203,15 @@ __global__ __launch_bounds__(THREADS) void mx_norm_kernel(float* __restrict__ re
 
 template <typename TD, typename TW, int BITS, bool ALIGNED>
 int mx_norm_launch(float* residual, const void* delta, int n_delta, int64_t delta_stride, const void* w, uint8_t* elements, uint8_t* scales,
-                   const int* rows, int n_rows, int width, int padded, float eps, hipStream_t s) {
+                   const int* rows, int n_rows, int width, int padded, float eps, bool many, hipStream_t s) {
 #define ARLE_MX_NORM(THREADS, VPT)                                                                                       \
   mx_norm_kernel<TD, TW, BITS, ALIGNED, THREADS, VPT><<<n_rows, THREADS, 0, s>>>(                                        \
       residual, static_cast<const TD*>(delta), n_delta, delta_stride, static_cast<const TW*>(w), elements, scales, rows, width, padded, eps)
-  // few rows: a group of columns a thread, so that a row's loads are one trip; many, which hide each other's trips: fewer waves that wait for each
-  // other's sums (us, one group a thread / two: 1,024 x 2,560 8.4 / 7.8, 2,048 x 2,560 13.5 / 12.8, 4,096 x 4,096 37.3 / 35.0, 600 x 4,096 8.3 /
-  // 7.8; level at 512 rows, and at 2,048 x 5,120 with four groups instead of two 26.1 / 26.8).  Past 8,192 columns four groups a thread: 2,048 x 12,288
-  // 42.7 us, 6.5 TB/s (52.3 where three parts ahead and the weight beside the row spill registers), 2,048 x 12,290, whose columns are loaded one by one,
-  // 76, one row of 12,288 with four parts 6.2
-  const bool many = n_rows > 512;
+  // few rows: a group of columns a thread, so that a row's loads are one trip; many (more than 512 in all), which hide each other's trips: fewer waves
+  // that wait for each other's sums (us, one group a thread / two: 1,024 x 2,560 8.4 / 7.8, 2,048 x 2,560 13.5 / 12.8, 4,096 x 4,096 37.3 / 35.0, 600 x
+  // 4,096 8.3 / 7.8; level at 512 rows, and at 2,048 x 5,120 with four groups instead of two 26.1 / 26.8).  Past 8,192 columns four groups a thread:
+  // 2,048 x 12,288 42.7 us, 6.5 TB/s (52.3 where three parts ahead and the weight beside the row spill registers), 2,048 x 12,290, whose columns are
+  // loaded one by one, 76, one row of 12,288 with four parts 6.2
   if (padded <= 1024)
     ARLE_MX_NORM(256, 1);
   else if (padded <= 2048)
@@ -234,9 +242,12 @@ extern "C" int arle_mx_quantize(const void* x, int code, long long ldx, void* el
   const int units = padded / 8, parts = (units + 511) / 512, threads = ((units + parts - 1) / parts + kWave - 1) / kWave * kWave;
   uint8_t* e = static_cast<uint8_t*>(elements);
   uint8_t* c = static_cast<uint8_t*>(scales);
-#define ARLE_MX_Q(T, BITS, ALIGNED, ROWS)                                                                                        \
-  mx_quantize_kernel<T, BITS, ALIGNED, ROWS><<<dim3((rows + ROWS - 1) / ROWS, parts), threads, 0, s>>>(static_cast<const T*>(x), ldx, e, c, \
-                                                                                                       rows, width, padded, threads)
+#define ARLE_MX_Q(T, BITS, ALIGNED, ROWS)                                                                                                        \
+  return mx_by_launches(rows, [&](int64_t at, int n) {                                                                                           \
+    mx_quantize_kernel<T, BITS, ALIGNED, ROWS><<<dim3((n + ROWS - 1) / ROWS, parts), threads, 0, s>>>(                                           \
+        static_cast<const T*>(x) + at * ldx, ldx, e + at * (padded * BITS / 8), c + at * (padded / kMxBlock), n, width, padded, threads);        \
+    return launch_status();                                                                                                                      \
+  })
 #define ARLE_MX_QR(T, BITS, ALIGNED)          \
   do {                                        \
     if (rows <= 1024)                         \
@@ -265,28 +276,24 @@ extern "C" int arle_mx_quantize(const void* x, int code, long long ldx, void* el
 #undef ARLE_MX_QA
 #undef ARLE_MX_QR
 #undef ARLE_MX_Q
-  return launch_status();
 }
 
 extern "C" int arle_mx_values(const void* elements, long long ld, const void* scales, long long ld_scales, int bits, void* out, int out_code,
                               int rows, int width, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int units = (width + 7) / 8, parts = (units + 511) / 512, threads = ((units + parts - 1) / parts + kWave - 1) / kWave * kWave;
-  const dim3 grid(rows, parts);
   const uint8_t* e = static_cast<const uint8_t*>(elements);
   const uint8_t* c = static_cast<const uint8_t*>(scales);
-  if (out_code == kF32) {
-    if (bits == kMx8)
-      mx_values_kernel<float, kMx8><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<float*>(out), width, threads);
-    else
-      mx_values_kernel<float, kMx4><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<float*>(out), width, threads);
-  } else {
-    if (bits == kMx8)
-      mx_values_kernel<bf16, kMx8><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<bf16*>(out), width, threads);
-    else
-      mx_values_kernel<bf16, kMx4><<<grid, threads, 0, s>>>(e, ld, c, ld_scales, static_cast<bf16*>(out), width, threads);
-  }
-  return launch_status();
+  const auto go = [&](auto t, auto b) {
+    using T = decltype(t);
+    return mx_by_launches(rows, [&](int64_t at, int n) {
+      mx_values_kernel<T, decltype(b)::value><<<dim3(n, parts), threads, 0, s>>>(e + at * ld, ld, c + at * ld_scales, ld_scales, static_cast<T*>(out) + at * width,
+                                                                                width, threads);
+      return launch_status();
+    });
+  };
+  const auto with_bits = [&](auto t) { return bits == kMx8 ? go(t, std::integral_constant<int, kMx8>{}) : go(t, std::integral_constant<int, kMx4>{}); };
+  return out_code == kF32 ? with_bits(float{}) : with_bits(bf16{});
 }
 
 extern "C" int arle_mx_add_rmsnorm(void* residual, const void* delta, int n_delta, long long delta_stride, int delta_code, const void* w,
@@ -294,9 +301,15 @@ extern "C" int arle_mx_add_rmsnorm(void* residual, const void* delta, int n_delt
                                    int aligned, float eps, void* stream) {
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto go = [&](auto td, auto tw, auto b, auto al) {
-    return mx_norm_launch<decltype(td), decltype(tw), decltype(b)::value, decltype(al)::value>(
-        static_cast<float*>(residual), delta, n_delta, delta_stride, w, static_cast<uint8_t*>(elements), static_cast<uint8_t*>(scales),
-        static_cast<const int*>(rows), n_rows, width, padded, eps, s);
+    using TD = decltype(td);
+    constexpr int kBits = decltype(b)::value;
+    return mx_by_launches(n_rows, [&](int64_t at, int n) {
+      const int64_t src = rows == nullptr ? at * width : 0;      // picked rows are anywhere in the residual
+      return mx_norm_launch<TD, decltype(tw), kBits, decltype(al)::value>(
+          static_cast<float*>(residual) + src, static_cast<const TD*>(delta) + src, n_delta, delta_stride, w,
+          static_cast<uint8_t*>(elements) + at * (padded * kBits / 8), static_cast<uint8_t*>(scales) + at * (padded / kMxBlock),
+          rows == nullptr ? nullptr : static_cast<const int*>(rows) + at, n, width, padded, eps, n_rows > 512, s);
+    });
   };
   auto with_align = [&](auto td, auto tw, auto b) { return aligned ? go(td, tw, b, std::true_type{}) : go(td, tw, b, std::false_type{}); };
   auto with_bits = [&](auto td, auto tw) {
