@@ -51,12 +51,12 @@ __device__ __forceinline__ mx_i32x8 mx_operand8(u32x4 a, u32x4 b) {
 // gate / (1 + exp(-gate)) * up, off by less than 2^-20 of itself for gates from -88.7 on (under which exp(-gate) leaves the floats and the result is 0).
 // exp(-gate) = 2^t (1 + r), t = -gate log2(e) rounded and r = -gate - t ln 2: without r the rounding of t is off by |gate| 2^-24 of the result, 2^-18 at
 // -80.  The quotient comes from the hardware's reciprocal of (1 + exp(-gate)) 2^-32: that of 1 + exp(-gate) itself would be under the smallest normal
-// float, for it 0, from -87.3 on.  t ends at -200, where 2^t is 0 already: an infinite one would make a gate of 2^128 / log2(e) none.
+// float, for it 0, from -87.3 on.  t ends at -200 and 200, where 2^t is 0 or an infinity already: past them r is none, or the -1 that makes an infinity none.
 // (us, with that rounding and those zeros, four operations less / so: gate|up of 4,096 x 12,288 x 4,096 292 / 295, with X in e2m1 204 / 210, 2,048 x
 // 9,728 x 2,560 87.8 / 89.5, up to 16 rows level; with expf and a whole quotient the activations of a workgroup's 256 x 128 results were a tenth of its time.)
 __device__ __forceinline__ float mx_silu_mul(float gate, float up) {
   constexpr float kLog2e = 1.44269502162933349609375f, kLn2 = 0.693147182464599609375f, kPart = 0x1p-32f;
-  const float t = fmaxf(gate * -kLog2e, -200.0f), r = fmaf(t, -kLn2, -gate);
+  const float t = __builtin_amdgcn_fmed3f(gate * -kLog2e, -200.0f, 200.0f), r = fmaf(t, -kLn2, -gate);
   const float d = fmaf(__builtin_amdgcn_exp2f(t), fmaf(r, kPart, kPart), kPart);
   return gate * (__builtin_amdgcn_rcpf(d) * kPart) * up;
 }

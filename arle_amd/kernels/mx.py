@@ -466,8 +466,9 @@ def _checked(x: MXRows, w: MXWeight, gated: bool) -> int:
 
 def gemm(x: MXRows, w: MXWeight, out_dtype: torch.dtype = torch.bfloat16, partials_ok: bool = False, *, variant: int | None = None,
          splits: int | None = None) -> torch.Tensor:
-    """x [T, K] . w [N, K]^T -> [T, N] in `out_dtype`, with sums of 32 bits behind what "mxfp8" rows lose inside every eight k (up to 7 * 2^-13 of its largest product:
-    see the module); with `partials_ok` possibly a float32 stack [S, T, N] whose sum over S, in order, is the product (as Linear's).  The sizes choose the kernel, or `variant` names it and `splits` its parts of K (default: 1)."""
+    """x [T, K] . w [N, K]^T -> [T, N] in `out_dtype`, with sums of 32 bits behind what "mxfp8" rows lose inside every eight k (up to 7 * 2^-13 of its
+    largest product: see the module); with `partials_ok` possibly a float32 stack [S, T, N] whose sum over S, in order, is the product (as Linear's).
+    The sizes choose the kernel, or `variant` names it and `splits` its parts of K (default: 1)."""
     device = _checked(x, w, False)
     code = _CODES.get(out_dtype)
     if code is None:

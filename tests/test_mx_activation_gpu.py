@@ -82,3 +82,23 @@ def test_gates_whose_exponential_is_near_the_largest_float(variant):
     wide[:, 0] = torch.tensor([1.0, 64.0])[torch.arange(64) % 2] * torch.where(torch.arange(64) < 32, 1.0, 2.0**-126)
     v = mx.values(mx.gate_up_act(mx.quantize(huge, "mxfp4"), mx.lay_weight(mx.quantize(wide.to(DEV), "mxfp4"), gated=True), variant=variant)).cpu()
     assert torch.equal(v[0], torch.tensor([2.0**114, 2.0**126])[torch.arange(32) % 2])
+
+
+@pytest.mark.parametrize("variant", [mx.GATED_ROWS, 3])
+def test_gates_that_are_far_below_zero(variant):
+    """Exponentials past the floats give zeros, whatever is left of -gate behind t ln 2 in 32 bits: at these gates it is -1, by which an infinity would be
+    multiplied as by zero."""
+    gates = [85764464, 132280784, 178797104, 202055264, 434636864, 481153184, 527669504, 3 * 2**24, 2**29]
+    blocks = 15
+    xe, xs = torch.zeros(len(gates), 32 * blocks, dtype=torch.uint8), torch.zeros(len(gates), blocks, dtype=torch.uint8)
+    for r, gate in enumerate(gates):
+        for b in range(blocks):                       # a digit to the base four a block
+            xe[r, 32 * b], xs[r, b] = (0, 10, 12, 13)[gate >> 2 * b & 3], 127 + 2 * b
+    w = torch.zeros(128, 32 * blocks)
+    w[:, ::32] = 1.0
+    w[64:, ::32] = 2.0**-10
+    rows = mx.rows_from_codes(xe.to(DEV), xs.to(DEV), 32 * blocks, "mxfp4")
+    plainly = mx.gemm(rows, mx.lay_weight(mx.quantize(w.to(DEV), "mxfp4")), torch.float32)
+    assert torch.equal(plainly[:, 0].cpu(), -torch.tensor(gates).float())
+    v = mx.values(mx.gate_up_act(rows, mx.lay_weight(mx.quantize(w.to(DEV), "mxfp4"), gated=True), variant=variant))
+    assert (v == 0).all()
